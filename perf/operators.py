@@ -54,8 +54,8 @@ def listed():
         _q4("q4_one", "f32", 1, 2304, 768, 64, True),
         # GPT-2 XL's first feed-forward product for eight sequences
         _q4("q4_step_8", "bf16", 8, 6400, 1600, 64, True),
-        # the widest product of a large layer for a step of 32 sequences
-        _q4("q4_wide_32", "bf16", 32, 28672, 8192, 128, False),
+        # the widest product of a large layer for a step of 16 sequences
+        _q4("q4_wide_16", "bf16", 16, 28672, 8192, 128, False),
         # the end of a step of 8 sequences: the drawn tokens' log probabilities and five alternatives each
         _logprobs("logprobs_step_8", "f32", 8, 50257, 5),
         # scoring of given text
@@ -96,7 +96,7 @@ def draw(rng):
         keep = rng.choice((0, 4, 70)) if window else 0
         case = _attend("", dtype, seqs, min(rows, context), context, kv_heads * group, kv_heads, dim, page, ragged, window, keep)
     elif op == "q4":
-        m, k = _log_int(rng, 1, 64), _log_int(rng, 64, 16384)
+        m, k = _log_int(rng, 1, 16), _log_int(rng, 64, 16384)
         case = _q4("", dtype, m, _log_int(rng, 16, min(32000, 16384 * 8192 // k)), k, rng.choice((64, 128)), rng.random() < 0.5)
     else:
         vocab = _log_int(rng, 1000, 160000)
@@ -182,7 +182,7 @@ def prepare(case, seed):
         codes = torch.randint(1, 16, (nt * 16, kt * 64), generator=g, device="cuda", dtype=torch.uint8)
         codes[n:] = 8
         codes[:, k:] = 8
-        c = codes.view(nt, 2, 8, kt, 4, 8, 2).permute(0, 3, 2, 4, 1, 5, 6)
+        c = codes.view(nt, 2, 8, kt, 4, 2, 8)[..., [0, 2, 4, 6, 1, 3, 5, 7]].view(nt, 2, 8, kt, 4, 2, 4, 2).permute(0, 3, 2, 4, 1, 5, 6, 7)
         s["packed"] = (c[..., 0] | c[..., 1] << 4).contiguous().view(nt, kt, 512)
         s["scales"] = (torch.rand(_cdiv(k, group), nt * 16, generator=g, device="cuda") * 0.01 + 0.002).to(torch.bfloat16)
         s["scales"][:, n:] = 0
@@ -364,8 +364,9 @@ def _plain_q4(s):
     c = s["case"]
     n, k, group = c["n"], c["k"], c["group"]
     nt, kt = s["packed"].shape[:2]
-    p = s["packed"].view(nt, kt, 8, 4, 2, 8)
-    w = torch.stack((p & 15, p >> 4), -1).permute(0, 4, 2, 1, 3, 5, 6).reshape(nt * 16, kt * 64)[:n, :k].float() - 8
+    p = s["packed"].view(nt, kt, 8, 4, 2, 2, 4)
+    w = torch.stack((p & 15, p >> 4), -1).flatten(-2)[..., [0, 4, 1, 5, 2, 6, 3, 7]].permute(0, 4, 2, 1, 3, 5, 6).reshape(nt * 16, kt * 64)
+    w = w[:n, :k].float() - 8
     w *= s["scales"].float().t()[:n].repeat_interleave(group, 1)[:, :k]
     out = s["x"].float() @ w.t()
     if s["bias"] is not None:
@@ -504,8 +505,9 @@ def _exact_q4(s):
     tile = torch.arange(k, device="cuda")
     for r in range(0, n, 2048):
         row = torch.arange(r, min(n, r + 2048), device="cuda")[:, None]
-        byte = (row % 8 * 4 + tile % 64 // 16) * 16 + row % 16 // 8 * 8 + tile % 16 // 2
-        code = s["packed"][row // 16, tile // 64, byte].long() >> 4 * (tile % 2) & 15
+        field = tile % 8 // 2 + tile % 2 * 4
+        byte = (row % 8 * 4 + tile % 64 // 16) * 16 + row % 16 // 8 * 8 + tile % 16 // 8 * 4 + field // 2
+        code = s["packed"][row // 16, tile // 64, byte].long() >> 4 * (field % 2) & 15
         out.append(s["x"].double() @ ((code - 8).double() * s["scales"][tile // c["group"], row].double()).t())
     out = torch.cat(out, 1)
     return out + s["bias"].double() if s["bias"] is not None else out
