@@ -342,6 +342,81 @@ int pg_decode_attention_noalloc(const float* d_qkv, float* d_out, float* d_kv_po
                                 int32_t n_head, int32_t head_dim, int32_t page_tokens,
                                 int32_t pages_per_seq, int32_t splits, int32_t device, void* stream);
 
+/* ------------------------------------------------------------------ serving operators on device buffers */
+/* None of these has a counterpart in the reference (FP32 weights and cache, logits on the host). Common rules:
+ *  - all pointers but the cache struct itself are DEVICE pointers of `device` that the caller owns; nothing is allocated;
+ *  - the call is enqueued on `stream` (a cudaStream_t, NULL = the default stream) and not waited for. It can be captured into
+ *    a CUDA graph once one call of any kind has been made on the device; sizes are fixed by the capture, what lies in device
+ *    memory (lengths, tables, row starts) is read anew by every replay;
+ *  - the calling thread's current device is restored before the call returns;
+ *  - sizes, strides (in elements) and alignments are checked and refused with PG_INVALID_INPUT; numbers in device memory cannot
+ *    be: what the kernels do with numbers out of range is said below, and is never an access outside the given buffers. */
+enum { PG_DTYPE_F32 = 0, PG_DTYPE_BF16 = 1 };
+
+/* One layer's keys and values in 8 bits. pool: [n_pages][kv_heads] blocks of 2 * page_tokens * padded bytes, padded = head_dim
+ * rounded up to 64: the keys [page_tokens][padded], then the values [padded][page_tokens], all e4m3 codes. scales:
+ * [n_pages][kv_heads][2] (keys, values): a code stands for code * scale. page_table: [seqs][pages_per_seq], the page of every
+ * page_tokens positions of a sequence. A page number outside 0..n_pages-1 is no page: nothing is written to it and its
+ * positions are not seen. Two sequences may share pages that neither appends to. */
+typedef struct {
+  void* pool;                 /* pg_kv8_pool_bytes() bytes, 16-byte aligned */
+  float* scales;
+  const int32_t* page_table;
+  int32_t n_pages, page_tokens /* 16, 32 or 64 */, kv_heads, head_dim /* even, 2..256 */, seqs /* 1..4096 */, pages_per_seq;
+  int32_t device;
+} pg_kv8_cache;
+uint64_t pg_kv8_pool_bytes(int32_t n_pages, int32_t page_tokens, int32_t kv_heads, int32_t head_dim);
+
+/* Appends the keys and values of `rows` new tokens, keys rotated by their positions on the way; queries of the same rows are
+ * rotated too where given. Sequence b has rows row_start[b]..row_start[b+1]-1 (row_start NULL: row b is sequence b's, rows =
+ * seqs) at the last positions of lens[b], its length WITH them. k, v: [rows][kv_heads][head_dim], q and q_out: [rows][heads]
+ * [head_dim], FP32 or BF16, each with its own distance between rows; q_out may be q. rot_dims (even, 0 = none): entry i of a head
+ * turns with entry i + rot_dims / 2 by position * rot_base^(-2i / rot_dims).
+ * The scale of a block (a page's keys or values of one head) is the smallest power of two (from 2^-100 up) that keeps its
+ * largest magnitude within 448, the largest e4m3 value; it grows with later tokens, whose append brings the block's earlier
+ * codes to the new scale (exact but for codes that become subnormal). The append that writes a page's first position starts
+ * the block anew. A NaN or an infinity makes the block's scale NaN: all its tokens read as NaN. Rows at positions below 0 or
+ * beyond the table are not stored. No two rows of a call may name the same position of a page. */
+int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const void* v, int64_t v_row, const void* q,
+                  int64_t q_row, void* q_out, int64_t q_out_row, int32_t dtype, int32_t heads, int32_t rows,
+                  const int32_t* row_start, const int32_t* lens, int32_t rot_dims, double rot_base, void* stream);
+
+/* out[row][head] = softmax(scale * q . k) v over the cached tokens that the row sees: those up to its own position, and with
+ * window > 0 only the last `window` of them (its own included) and the first keep_first of the sequence. Rows belong to sequences
+ * as in pg_kv8_append, whose `lens` it takes; query head h reads key / value head h / (heads / kv_heads). A row that sees nothing
+ * gets zeros; rows outside row_start[0]..row_start[seqs]-1 are left as they were. max_rows: at least the rows of any sequence
+ * (it chooses the kernels; a sequence with more is still computed). FP32 queries are computed to FP32 grade from pairs of
+ * FP16 numbers, BF16 queries with FP16 probabilities; sums are FP32.
+ * workspace: pg_kv8_attention_workspace_bytes() bytes, 256-byte aligned, zeroed by the caller before its first use and left ready for the next
+ * call. Calls that may overlap on the GPU (captured graphs among them) need workspaces of their own. */
+uint64_t pg_kv8_attention_workspace_bytes(const pg_kv8_cache* cache, int32_t rows, int32_t heads, int32_t dtype);
+int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, void* out, int64_t out_row, int32_t dtype,
+                     int32_t heads, int32_t rows, int32_t max_rows, const int32_t* row_start, const int32_t* lens, float scale,
+                     int32_t window, int32_t keep_first, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* 4-bit weights. A matrix [n][k] is held as unsigned codes (weight = (code - 8) * scale) with one BF16 scale for every `group` (64 or
+ * 128) inputs of an output. packed: [ceil(n/16)][ceil(k/64)] tiles of 512 bytes; in a tile output r and inputs 16c..16c+15 are
+ * the 8 bytes from ((r % 8) * 4 + c) * 16 + (r / 8) * 8 on, two words of 8 inputs each, whose 4-bit field i holds input 2i (i < 4) or
+ * 2(i - 4) + 1. Places behind the matrix hold 8. scales: [ceil(k/group)][16 * ceil(n/16)], 0 behind the matrix. */
+uint64_t pg_q4_packed_bytes(int32_t n, int32_t k);
+uint64_t pg_q4_scale_bytes(int32_t n, int32_t k, int32_t group);
+/* scale = bf16(max |w| / 7) of the group, code = 8 + w / scale rounded to nearest (ties to even) and kept in 0..15. w: [n][k] finite FP32 or BF16. */
+int pg_quantize_q4(const void* w, int64_t w_row, int32_t dtype, int32_t n, int32_t k, int32_t group, void* packed, void* scales,
+                   int32_t device, void* stream);
+/* out[m][n] = x[m][k] . dequant(w)[n][k]^T + bias; 1 <= m <= 16; x, bias (may be NULL) and out FP32 or BF16. FP32 inputs are
+ * computed to FP32 grade from pairs of FP16 numbers. */
+int pg_linear_q4(const void* x, int64_t x_row, const void* packed, const void* scales, const void* bias, int32_t dtype, int32_t m,
+                 int32_t n, int32_t k, int32_t group, void* out, int64_t out_row, int32_t device, void* stream);
+
+/* Scores of the rows of logits [rows][vocab] (FP32 or BF16): logprobs[row] = log softmax(logits[row])[targets[row]], entropy[row] =
+ * -sum p log p (0 log 0 = 0), and the top_k (0..32) largest log probabilities with their ids, largest first, equal ones by
+ * the lower id. targets and logprobs may both be NULL, and so may entropy. A target of -1 gives 0, any other outside 0..vocab-1
+ * NaN. Entries of -infinity have probability 0. A row with a NaN or +infinity, or with nothing but -infinity, has no
+ * distribution: NaN everywhere, ids -1. */
+int pg_token_logprobs(const void* logits, int64_t row, int32_t dtype, int32_t rows, int32_t vocab, const int32_t* targets,
+                      float* logprobs, float* entropy, int32_t top_k, int32_t* top_ids, float* top_logprobs, int32_t device,
+                      void* stream);
+
 /* ------------------------------------------------------------------ generation loops */
 /* non-zero return aborts generation (the closure returning Err in the reference) */
 typedef int (*pg_token_callback)(uint64_t token_id, void* user);

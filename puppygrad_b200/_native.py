@@ -46,6 +46,11 @@ class PgOperationProfile(C.Structure):
                [("launches", C.c_uint64 * 8), ("fused_step_kernel", C.c_double), ("fused_phases", C.c_uint64)]
 
 
+class PgKv8Cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("pool", "scales", "page_table")] + \
+               [(n, C.c_int32) for n in ("n_pages", "page_tokens", "kv_heads", "head_dim", "seqs", "pages_per_seq", "device")]
+
+
 TOKEN_CALLBACK = C.CFUNCTYPE(C.c_int, C.c_uint64, C.c_void_p)
 DECODE_TOKENS_FN = C.CFUNCTYPE(C.c_int, C.POINTER(C.c_uint64), C.c_size_t, C.POINTER(C.c_char), C.c_size_t,
                                C.POINTER(C.c_size_t), C.c_void_p)
@@ -106,6 +111,18 @@ SIGNATURES = {
                                   C.c_int32, _fp, C.POINTER(C.c_double)]),
     "pg_decode_attention_noalloc": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                               C.c_int32, C.c_int32, C.c_int32, _vp]),
+    "pg_kv8_pool_bytes": (C.c_uint64, [C.c_int32] * 4),
+    "pg_kv8_append": (C.c_int, [C.POINTER(PgKv8Cache), _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, C.c_int32, C.c_int32,
+                                C.c_int32, _vp, _vp, C.c_int32, C.c_double, _vp]),
+    "pg_kv8_attention_workspace_bytes": (C.c_uint64, [C.POINTER(PgKv8Cache), C.c_int32, C.c_int32, C.c_int32]),
+    "pg_kv8_attention": (C.c_int, [C.POINTER(PgKv8Cache), _vp, C.c_int64, _vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp,
+                                   C.c_float, C.c_int32, C.c_int32, _vp, C.c_uint64, _vp]),
+    "pg_q4_packed_bytes": (C.c_uint64, [C.c_int32] * 2),
+    "pg_q4_scale_bytes": (C.c_uint64, [C.c_int32] * 3),
+    "pg_quantize_q4": (C.c_int, [_vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, C.c_int32, _vp]),
+    "pg_linear_q4": (C.c_int, [_vp, C.c_int64, _vp, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, C.c_int64, C.c_int32,
+                               _vp]),
+    "pg_token_logprobs": (C.c_int, [_vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int32, _vp, _vp, C.c_int32, _vp]),
     "pg_generate_greedy": (C.c_int, [_vp, _ip, C.c_int32, C.c_uint64, _ip, _u64p]),
     "pg_stream_greedy_tokens": (C.c_int, [_vp, _ip, C.c_int32, C.c_uint64, TOKEN_CALLBACK, _vp, _ip, _u64p]),
     "pg_generate_with_config": (C.c_int, [_vp, _ip, C.c_int32, C.POINTER(PgGenerationConfig), TOKEN_CALLBACK,

@@ -1,0 +1,46 @@
+// What the kernels over the 8-bit cache share: rows of a sequence, pages, conversions.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "device_util.cuh"
+#include "serving.h"
+
+namespace pg {
+namespace {
+
+// Rows [first, first + n) of sequence b. Whatever row_start holds, they lie within the call's rows.
+struct SeqRows {
+  int first, n;
+};
+__device__ __forceinline__ SeqRows seq_rows(const int* row_start, int rows, int b) {
+  if (!row_start) return {b, 1};
+  const int r0 = min(max(row_start[b], 0), rows), r1 = min(max(row_start[b + 1], r0), rows);
+  return {r0, r1 - r0};
+}
+
+// Page of logical page `lp` of sequence b, -1 where there is none.
+__device__ __forceinline__ int page_of(const Kv8View& c, int b, int lp) {
+  if (lp < 0 || lp >= c.pages_per_seq) return -1;
+  const int page = c.table[(size_t)b * c.pages_per_seq + lp];
+  return (unsigned)page < (unsigned)c.n_pages ? page : -1;
+}
+
+// Two e4m3 codes (low and high byte) as FP16, exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(r) : "r"(two));
+  return r;
+}
+// Rounded to nearest even, kept within +-448; `a` in the low byte.
+__device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float a, float b) {
+  uint32_t r;
+  asm("{\n.reg .b16 t;\ncvt.rn.satfinite.e4m3x2.f32 t, %2, %1;\ncvt.u32.u16 %0, t;\n}" : "=r"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t f32x4_to_e4m3x4(float a, float b, float c, float d) {
+  return f32x2_to_e4m3x2(a, b) | f32x2_to_e4m3x2(c, d) << 16;
+}
+
+}  // namespace
+}  // namespace pg

@@ -1,0 +1,75 @@
+// Launches of the serving operators on device buffers (serving.cu has the entry points and their checks).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "puppygrad_b200.h"
+
+namespace pg {
+
+constexpr int KV8_MAX_SEQS = 4096;
+constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace must not hang on the device
+
+__host__ __device__ inline int kv8_padded(int head_dim) { return (head_dim + 63) / 64 * 64; }
+
+// The cache as the kernels see it.
+struct Kv8View {
+  uint8_t* pool;
+  float* scales;
+  const int* table;
+  int n_pages, page_tokens, page_shift, kv_heads, dim, seqs, pages_per_seq;
+};
+struct Kv8AppendArgs {
+  Kv8View c;
+  const void *k, *v, *q;
+  void* q_out;
+  int64_t k_row, v_row, q_row, q_out_row;
+  int heads, rows;
+  const int *row_start, *lens;
+  int rot_dims;
+  double turn_step;  // entry i turns by position * 2^(turn_step * i)
+};
+struct Kv8AttnArgs {
+  Kv8View c;
+  const void* q;
+  void* out;
+  int64_t q_row, out_row;
+  int heads, group, rows, max_rows;
+  const int *row_start, *lens;
+  float scale;
+  int window, keep;
+  unsigned* counters;
+  float* partials;
+};
+struct Q4Args {
+  const void *x, *bias;
+  const uint8_t* packed;
+  const uint16_t* scales;
+  void* out;
+  int64_t x_row, out_row;
+  int m, n, k, group;
+};
+struct LogprobArgs {
+  const void* logits;
+  int64_t row;
+  int rows, vocab, top_k;
+  const int* targets;
+  float *logprobs, *entropy;
+  int* top_ids;
+  float* top_logprobs;
+};
+
+// Rows of a tile of the step kernel: FP32 queries take two MMA rows each.
+inline int kv8_tile_rows(int dtype) { return dtype == PG_DTYPE_F32 ? 8 : 16; }
+
+cudaError_t init_kv8_append_attributes();
+cudaError_t init_kv8_step_attributes();
+cudaError_t init_q4_attributes();
+cudaError_t launch_kv8_append(const Kv8AppendArgs& a, int dtype, cudaStream_t s);
+cudaError_t launch_kv8_attention_step(const Kv8AttnArgs& a, int dtype, int sms, cudaStream_t s);
+cudaError_t launch_quantize_q4(const void* w, int64_t w_row, int dtype, int n, int k, int group, uint8_t* packed, uint16_t* scales, cudaStream_t s);
+cudaError_t launch_linear_q4(const Q4Args& a, int dtype, int sms, cudaStream_t s);
+cudaError_t launch_token_logprobs(const LogprobArgs& a, int dtype, int sms, cudaStream_t s);
+
+}  // namespace pg

@@ -1,0 +1,177 @@
+"""Operators of a serving program on its own device buffers: a paged cache of keys and values in 8 bits, products with 4-bit weights, log
+probabilities of given tokens. include/puppygrad_b200.h has the layouts and what each call promises.
+
+Buffers are anything with the interface of a torch tensor (`data_ptr`, `shape`, `stride`, `dtype`, `device`); torch itself is not
+imported. Calls are enqueued on `stream` (a CUDA stream's address, 0 = the default stream) and return without waiting; what they
+read must stay allocated until they have run.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+from . import _native as N
+from .errors import Gpt2Error, check
+
+_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1}
+
+
+def _bad(what: str):
+    return Gpt2Error("InvalidInput", what)
+
+
+def _code(t, name: str) -> int:
+    code = _DTYPES.get(str(t.dtype))
+    if code is None:
+        raise _bad(f"{name}: dtype {t.dtype} must be float32 or bfloat16")
+    return code
+
+
+def _device(t, name: str) -> int:
+    if t.device.type != "cuda":
+        raise _bad(f"{name} is on {t.device}, a CUDA device is needed")
+    return t.device.index
+
+
+def _flat(t, name: str, dtype: str, shape: Tuple[int, ...], device: int) -> int:
+    """Address of a buffer that has to be contiguous and of that type and shape."""
+    if str(t.dtype) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise _bad(f"{name}: {dtype} {shape} without gaps is needed, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    if _device(t, name) != device:
+        raise _bad(f"{name} is on {t.device}, the others are on cuda:{device}")
+    return t.data_ptr()
+
+
+def _rows(t, name: str, dtype, inner: Tuple[int, ...], device: int, rows: Optional[int] = None) -> Tuple[int, int]:
+    """Address and distance between rows of [rows, *inner], whose rows are without gaps."""
+    shape, stride = tuple(t.shape), t.stride()
+    if shape[1:] != inner or (rows is not None and shape[0] != rows) or t.dtype != dtype:
+        raise _bad(f"{name}: {dtype} [{'rows' if rows is None else rows}, {', '.join(map(str, inner))}] is needed, got {t.dtype} {shape}")
+    width = 1
+    for n, s in zip(reversed(inner), reversed(stride[1:])):
+        if n > 1 and s != width:
+            raise _bad(f"{name}: a row must be without gaps, got strides {stride}")
+        width *= n
+    if _device(t, name) != device:
+        raise _bad(f"{name} is on {t.device}, the others are on cuda:{device}")
+    # of a single row (or none) the distance says nothing
+    return t.data_ptr(), stride[0] if shape[0] > 1 else width
+
+
+class Kv8Cache:
+    """One layer's keys and values in 8 bits, in buffers of the caller: `pool` uint8 [n_pages, kv_heads, 2 * page_tokens * padded] with
+    padded = head_dim rounded up to 64, `scales` float32 [n_pages, kv_heads, 2], `page_table` int32 [seqs, pages_per_seq]. The object
+    holds references to them and nothing of their contents: pages are handed out by writing page_table."""
+
+    def __init__(self, pool, scales, page_table, page_tokens: int, head_dim: int):
+        device = _device(pool, "pool")
+        if len(pool.shape) != 3 or len(page_table.shape) != 2:
+            raise _bad(f"pool {tuple(pool.shape)} and page_table {tuple(page_table.shape)} must have 3 and 2 dimensions")
+        n_pages, kv_heads = pool.shape[:2]
+        self._c = N.PgKv8Cache()
+        self._c.pool = _flat(pool, "pool", "torch.uint8", self.pool_shape(n_pages, kv_heads, page_tokens, head_dim), device)
+        self._c.scales = _flat(scales, "scales", "torch.float32", (n_pages, kv_heads, 2), device)
+        self._c.page_table = _flat(page_table, "page_table", "torch.int32", tuple(page_table.shape), device)
+        self._c.n_pages, self._c.page_tokens, self._c.kv_heads, self._c.head_dim = n_pages, page_tokens, kv_heads, head_dim
+        self._c.seqs, self._c.pages_per_seq, self._c.device = page_table.shape[0], page_table.shape[1], device
+        self.pool, self.scales, self.page_table = pool, scales, page_table
+        self.kv_heads, self.head_dim, self.seqs, self.device = kv_heads, head_dim, page_table.shape[0], device
+        self._ref = C.byref(self._c)
+
+    @staticmethod
+    def pool_shape(n_pages: int, kv_heads: int, page_tokens: int, head_dim: int) -> Tuple[int, int, int]:
+        size = N.lib.pg_kv8_pool_bytes(n_pages, page_tokens, kv_heads, head_dim)
+        if not size:
+            raise _bad(N.lib.pg_last_error_message().decode())
+        return n_pages, kv_heads, size // (n_pages * kv_heads)
+
+    def _row_map(self, lens, row_start) -> Tuple[int, int]:
+        return (_flat(lens, "lens", "torch.int32", (self.seqs,), self.device),
+                0 if row_start is None else _flat(row_start, "row_start", "torch.int32", (self.seqs + 1,), self.device))
+
+    def append(self, k, v, lens, row_start=None, q=None, q_out=None, rot_dims: int = 0, rot_base: float = 10000.0, stream: int = 0) -> None:
+        """Appends k and v [rows, kv_heads, head_dim], k turned by its positions; q [rows, heads, head_dim] is turned into q_out (which
+        may be q). Sequence b has rows row_start[b] : row_start[b + 1] (None: row b), at the last positions of lens[b], its
+        length with them."""
+        rows, inner, device = k.shape[0], (self.kv_heads, self.head_dim), self.device
+        dtype = _code(k, "k")
+        kp, ks = _rows(k, "k", k.dtype, inner, device)
+        vp, vs = _rows(v, "v", k.dtype, inner, device, rows)
+        qp = qs = op = os = heads = 0
+        if q is not None or q_out is not None:
+            if q is None or q_out is None:
+                raise _bad("q and q_out must be given together")
+            heads = q.shape[1]
+            qp, qs = _rows(q, "q", k.dtype, (heads, self.head_dim), device, rows)
+            op, os = _rows(q_out, "q_out", k.dtype, (heads, self.head_dim), device, rows)
+        lp, sp = self._row_map(lens, row_start)
+        check(N.lib.pg_kv8_append(self._ref, kp, ks, vp, vs, qp, qs, op, os, dtype, heads, rows, sp, lp, rot_dims, rot_base, stream))
+
+    def workspace_bytes(self, rows: int, heads: int, dtype) -> int:
+        """Size of the workspace of `attention` calls of up to that many rows; its memory must be zero before its first use."""
+        code = _DTYPES.get(str(dtype), -1)
+        size = N.lib.pg_kv8_attention_workspace_bytes(self._ref, rows, heads, code)
+        if not size:
+            raise _bad(N.lib.pg_last_error_message().decode())
+        return size
+
+    def attention(self, q, out, lens, workspace, row_start=None, max_rows: int = 1, scale: Optional[float] = None, window: int = 0,
+                  keep_first: int = 0, stream: int = 0) -> None:
+        """out = softmax(scale * q . k) v over what each row sees; q and out [rows, heads, head_dim], scale head_dim ** -0.5 unless
+        given, `lens` and `row_start` as in `append`. max_rows: at least the rows of any sequence. `workspace`: uint8, zeroed
+        before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each."""
+        rows, heads = q.shape[0], q.shape[1]
+        dtype, inner = _code(q, "q"), (heads, self.head_dim)
+        qp, qs = _rows(q, "q", q.dtype, inner, self.device)
+        op, os = _rows(out, "out", q.dtype, inner, self.device, rows)
+        lp, sp = self._row_map(lens, row_start)
+        wp = _flat(workspace, "workspace", "torch.uint8", (workspace.shape[0],), self.device)
+        check(N.lib.pg_kv8_attention(self._ref, qp, qs, op, os, dtype, heads, rows, max_rows, sp, lp,
+                                     self.head_dim ** -0.5 if scale is None else scale, window, keep_first, wp, workspace.shape[0], stream))
+
+
+def q4_shapes(n: int, k: int, group: int) -> Tuple[Tuple[int, int, int], Tuple[int, int]]:
+    """Shapes of the packed codes (uint8) and the scales (bfloat16) of a 4-bit matrix of n outputs and k inputs."""
+    size = N.lib.pg_q4_scale_bytes(n, k, group)
+    if not size:
+        raise _bad(N.lib.pg_last_error_message().decode())
+    return (-(-n // 16), -(-k // 64), 512), (-(-k // group), -(-n // 16) * 16)
+
+
+def quantize_q4(w, packed, scales, group: int, stream: int = 0) -> None:
+    """Lays the matrix w [n, k] out in 4 bits, with one scale for every `group` (64 or 128) inputs of an output."""
+    n, k = w.shape
+    dtype, device = _code(w, "w"), _device(w, "w")
+    wp, ws = _rows(w, "w", w.dtype, (k,), device)
+    ps, ss = q4_shapes(n, k, group)
+    check(N.lib.pg_quantize_q4(wp, ws, dtype, n, k, group, _flat(packed, "packed", "torch.uint8", ps, device),
+                               _flat(scales, "scales", "torch.bfloat16", ss, device), device, stream))
+
+
+def linear_q4(x, packed, scales, out, group: int, bias=None, stream: int = 0) -> None:
+    """out [m, n] = x [m, k] @ dequant(w [n, k]).T + bias for up to 16 rows."""
+    m, k = x.shape
+    n = out.shape[1]
+    dtype, device = _code(x, "x"), _device(x, "x")
+    xp, xs = _rows(x, "x", x.dtype, (k,), device)
+    op, os = _rows(out, "out", x.dtype, (n,), device, m)
+    ps, ss = q4_shapes(n, k, group)
+    bp = 0 if bias is None else _flat(bias, "bias", str(x.dtype), (n,), device)
+    check(N.lib.pg_linear_q4(xp, xs, _flat(packed, "packed", "torch.uint8", ps, device), _flat(scales, "scales", "torch.bfloat16", ss, device), bp,
+                             dtype, m, n, k, group, op, os, device, stream))
+
+
+def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=None, top_logprobs=None, stream: int = 0) -> None:
+    """Scores of the rows of logits [rows, vocab]: logprobs [rows] of `targets` [rows], entropy [rows], the most likely ids and their
+    log probabilities [rows, k] (k up to 32), each where its output is given."""
+    rows, vocab = logits.shape
+    dtype, device = _code(logits, "logits"), _device(logits, "logits")
+    lp, ls = _rows(logits, "logits", logits.dtype, (vocab,), device)
+    if (top_ids is None) != (top_logprobs is None):
+        raise _bad("top_ids and top_logprobs must be given together")
+    k = 0 if top_ids is None else top_ids.shape[1]
+    f = lambda t, name, kind, shape: 0 if t is None else _flat(t, name, kind, shape, device)
+    check(N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, f(targets, "targets", "torch.int32", (rows,)),
+                                  f(logprobs, "logprobs", "torch.float32", (rows,)), f(entropy, "entropy", "torch.float32", (rows,)), k,
+                                  f(top_ids, "top_ids", "torch.int32", (rows, k)), f(top_logprobs, "top_logprobs", "torch.float32", (rows, k)),
+                                  device, stream))

@@ -1,0 +1,614 @@
+"""Serving operators on device buffers against their definitions in 64 bits.
+
+Tolerances, with u = half a step of a type relative to a value (FP32 2^-24, BF16 2^-8, e4m3 2^-4):
+ * attention, |v| <= V, scores within +-16 in the tests: an FP32 score is off by a few u of its size, 16 * 2^-20 in all with the pairs' rests
+   (2^-22) and the sum over the entries, which is the relative error of a weight; the weighted mean is off by twice that times V: 2^-15 V.
+   BF16 queries: weights rounded to FP16 (2^-11 of the largest weight each, in numerator only): 2^-10 V, and the result's own rounding.
+ * 4-bit products: operands are exact (FP32: within 2^-21 of the tile's largest input), sums FP32: 2^-18 sum |x w|, and the result's rounding.
+ * log probabilities: FP32 sums and logarithms, values up to 40 or so: 2^-18 * (1 + |value|).
+"""
+import math
+
+import pytest
+import torch
+
+import puppygrad_b200 as pg
+from tests import serving_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def starts(rows):
+    out = [0]
+    for n in rows:
+        out.append(out[-1] + n)
+    return i32(out)
+
+
+class Cache:
+    """A pool with codes of earlier tokens; bytes and scales that no live token owns are 0xFF, NaN."""
+
+    def __init__(self, lens, kvh, dim, page, seed, spread=2, spare=3, per_seq=None):
+        g = gen(seed)
+        used = [-(-n // page) for n in lens]
+        self.page, self.dim, self.kvh, self.lens = page, dim, kvh, lens
+        n_pages, per_seq = sum(used) + spare, per_seq or max(1, max(used)) + 1
+        self.pool = torch.full(pg.Kv8Cache.pool_shape(n_pages, kvh, page, dim), 255, dtype=torch.uint8, device=DEV)
+        self.scales = torch.full((n_pages, kvh, 2), math.nan, device=DEV)
+        self.table = torch.full((len(lens), per_seq), -1, dtype=torch.int32, device=DEV)
+        order, at = torch.randperm(n_pages, generator=g, device=DEV).tolist(), 0
+        k, v = ref.blocks(self.pool, page, dim)
+        for b, n in enumerate(lens):
+            for i in range(used[b]):
+                p, live = order[at], min(page, n - i * page)
+                at += 1
+                self.table[b, i] = p
+                values = (torch.randn(2, kvh, live, dim, generator=g, device=DEV) * 100).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+                k[p, :, :live] = 0
+                k[p, :, :live, :dim] = values[0]
+                v[p, :, :dim, :live] = values[1].transpose(-1, -2)
+                self.scales[p] = torch.exp2(torch.randint(-8, -8 + spread, (kvh, 2), generator=g, device=DEV).float())
+        self.handle = pg.Kv8Cache(self.pool, self.scales, self.table, page_tokens=page, head_dim=dim)
+
+    def kv(self, b, length=None):
+        return ref.sequence_kv(self.pool, self.scales, self.table[b], self.lens[b] if length is None else length, self.page, self.dim)
+
+
+def workspace(cache, rows, heads, dtype):
+    return torch.zeros(cache.handle.workspace_bytes(rows, heads, dtype), dtype=torch.uint8, device=DEV)
+
+
+def check_attention(cache, q, out, rows, scale, window=0, keep=0):
+    at = 0
+    for b, n in enumerate(rows):
+        length = cache.lens[b]
+        keys, values = cache.kv(b)
+        want = ref.attention(q[at:at + n].double(), keys, values, torch.arange(length - n, length, device=DEV), scale, window, keep)
+        got, u = out[at:at + n].double(), U[q.dtype]
+        top = float(values.abs().max()) if length else 0.0
+        tol = top * (2.0 ** -15 if q.dtype == F32 else 2.0 ** -10) + u * want.abs()
+        assert torch.isfinite(got).all(), (b, n, length)
+        assert ((got - want).abs() <= tol).all(), (b, n, length, float(((got - want).abs() - tol).max()), top)
+        at += n
+
+
+ATTENTION = [
+    # lens, rows, heads, kv heads, dim, page, window, keep
+    ([1], [1], 1, 1, 64, 16, 0, 0),
+    ([777], [1], 12, 12, 64, 32, 0, 0),
+    ([0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 500], [1] * 16, 8, 2, 64, 16, 0, 0),
+    ([0, 1, 16, 63, 64, 65, 129, 1000], [1] * 8, 10, 2, 96, 32, 0, 0),
+    ([300, 1, 64, 2000], [1] * 4, 32, 2, 128, 64, 0, 0),
+    ([130, 70], [1, 1], 48, 2, 80, 64, 0, 0),  # 24 rows for a head: more than a tile
+    ([5000], [1], 4, 1, 256, 64, 0, 0),
+    ([333, 90], [1, 1], 6, 3, 192, 16, 0, 0),
+    ([40, 70], [1, 1], 3, 3, 2, 16, 0, 0),
+    ([700, 64, 0, 130], [5, 64, 0, 3], 8, 2, 128, 64, 0, 0),
+    ([200, 3, 90], [7, 5, 1], 4, 4, 32, 32, 0, 0),  # more rows than tokens: the first see nothing
+    ([1000, 100, 64, 10], [1] * 4, 8, 4, 64, 64, 50, 0),
+    ([1000, 300, 64, 10], [3, 200, 64, 2], 8, 4, 64, 16, 100, 70),
+    ([1000, 131], [1, 60], 4, 1, 128, 32, 1, 0),  # each row sees itself alone
+    ([900], [1], 4, 4, 64, 64, 1000, 5),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens,rows,heads,kvh,dim,page,window,keep", ATTENTION)
+def test_attention(lens, rows, heads, kvh, dim, page, window, keep, dtype):
+    cache = Cache(lens, kvh, dim, page, 11 + sum(lens))
+    n, scale = sum(rows), dim ** -0.5
+    q = torch.randn(n, heads, dim, generator=gen(3), device=DEV).to(dtype)
+    out = torch.full((n + 2, heads, dim), 7.0, device=DEV, dtype=dtype)  # two rows behind the last sequence
+    ws = workspace(cache, n, heads, dtype)
+    one = all(r == 1 for r in rows)
+    for call in range(2):  # the workspace is left as it was
+        cache.handle.attention(q, out[:n], i32(lens), ws, row_start=None if one else starts(rows), max_rows=max(rows), window=window, keep_first=keep)
+        check_attention(cache, q, out[:n], rows, scale, window, keep)
+    assert (out[n:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_long_sequences_are_shared_out_over_all_blocks(dtype):
+    lens = [70001, 3, 20000]
+    cache = Cache(lens, 2, 64, 64, 5)
+    q = torch.randn(3, 8, 64, generator=gen(4), device=DEV).to(dtype)
+    out, ws = torch.empty_like(q), workspace(cache, 3, 8, dtype)
+    cache.handle.attention(q, out, i32(lens), ws)
+    check_attention(cache, q, out, [1, 1, 1], 64 ** -0.5)
+    again = torch.empty_like(q)
+    cache.handle.attention(q, again, i32(lens), ws)
+    assert torch.equal(out, again)  # the order of the parts is fixed
+
+
+def test_attention_many_sequences():
+    lens = [(i * 37) % 90 for i in range(700)]
+    cache = Cache(lens, 1, 64, 16, 6)
+    q = torch.randn(700, 2, 64, generator=gen(4), device=DEV)
+    out = torch.empty_like(q)
+    cache.handle.attention(q, out, i32(lens), workspace(cache, 700, 2, F32))
+    check_attention(cache, q, out, [1] * 700, 0.125)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_blocks_of_very_different_scales(dtype):
+    """The largest weight may belong to a block whose values are 2^40 times smaller than another block's."""
+    cache = Cache([256], 1, 64, 64, 8)
+    cache.scales[cache.table[0, 0].long()] = torch.tensor([2.0 ** -7, 2.0 ** -45], device=DEV)
+    cache.scales[cache.table[0, 2].long()] = torch.tensor([0.0, 2.0 ** -100], device=DEV)
+    q = torch.randn(1, 4, 64, generator=gen(9), device=DEV).to(dtype)
+    keys, values = cache.kv(0)
+    q[0, 0] = (keys[5, 0] * 8).to(dtype)  # head 0 looks at a token of the first block alone
+    out = torch.empty_like(q)
+    cache.handle.attention(q, out, i32([256]), workspace(cache, 1, 4, dtype))
+    check_attention(cache, q, out, [1], 0.125)
+    q2 = q[:, :1].contiguous()
+    out2 = torch.empty_like(q2)
+    cache.handle.attention(q2, out2, i32([40]), workspace(cache, 1, 1, dtype))  # the first block alone: tiny values, whole precision
+    want = ref.attention(q2.double(), keys[:40], values[:40], torch.tensor([39], device=DEV), 0.125)
+    assert ((out2.double() - want).abs() <= (2.0 ** -15 if dtype == F32 else 2.0 ** -10) * values[:40].abs().max() + U[dtype] * want.abs()).all()
+
+
+def test_attention_pages_that_are_none_and_lengths_beyond_the_table():
+    cache = Cache([300, 200], 2, 64, 32, 12)
+    cache.table[0, 3] = -1
+    cache.table[0, 4] = 10 ** 6
+    q = torch.randn(2, 4, 64, generator=gen(1), device=DEV)
+    out, ws = torch.empty_like(q), workspace(cache, 2, 4, F32)
+    lens = i32([300, 10 ** 6])
+    cache.handle.attention(q, out, lens, ws)
+    table = cache.table.clone()
+    cache.table.clamp_(0, cache.pool.shape[0] - 1)
+    keys, values = cache.kv(0)
+    gone = (torch.arange(300, device=DEV) >= 96) & (torch.arange(300, device=DEV) < 160)
+    want = ref.attention(q[:1].double(), keys, values, torch.tensor([299], device=DEV), 0.125, missing=gone)
+    assert ((out[:1].double() - want).abs() <= 2.0 ** -15 * values.abs().max() + 2.0 ** -24 * want.abs()).all()
+    # of the second sequence the table's pages are seen, all but those that are none
+    known = int((table[1] >= 0).sum()) * 32
+    assert known == 224
+    keys, values = cache.kv(1, known)  # tokens 200..223 of the last page hold NaN bytes: they count as stored
+    assert torch.isnan(values).any() and torch.isnan(out[1]).any()
+
+
+def test_attention_rows_outside_every_sequence_are_left():
+    cache = Cache([50, 60], 1, 64, 16, 2)
+    q = torch.randn(9, 2, 64, generator=gen(1), device=DEV)
+    out, ws = torch.full_like(q, 5.0), workspace(cache, 9, 2, F32)
+    cache.handle.attention(q, out, i32([50, 60]), ws, row_start=i32([2, 4, 7]), max_rows=3)
+    assert (out[:2] == 5).all() and (out[7:] == 5).all()
+    check_attention(cache, q[2:7], out[2:7], [2, 3], 0.125)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_rows_with_gaps_and_odd_addresses(dtype):
+    cache = Cache([500, 77], 2, 80, 16, 21)
+    wide = torch.randn(2, 4 * 80 + 13, generator=gen(2), device=DEV).to(dtype)
+    q = wide[:, 3:3 + 320].view(2, 4, 80)
+    big = torch.full((2, 4 * 80 + 7), 9.0, device=DEV, dtype=dtype)
+    out = big[:, 1:321].view(2, 4, 80)
+    cache.handle.attention(q, out, i32([500, 77]), workspace(cache, 2, 4, dtype))
+    check_attention(cache, q, out, [1, 1], 80 ** -0.5)
+    assert (big[:, 0] == 9).all() and (big[:, 321:] == 9).all()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_attention_queries_far_from_one(size):
+    cache = Cache([300], 1, 64, 16, 3)
+    q = torch.randn(1, 2, 64, generator=gen(1), device=DEV)
+    out, ws = torch.empty_like(q), workspace(cache, 1, 2, F32)
+    want = torch.empty_like(q)
+    cache.handle.attention(q, want, i32([300]), ws)
+    cache.handle.attention(q * size, out, i32([300]), ws, scale=0.125 / size)
+    check_attention(cache, q, out, [1], 0.125)
+
+
+# ------------------------------------------------------------------ append
+def quantised(x, scale):
+    """Half a step around each value: how far a code times its scale may be from x (both float64)."""
+    return scale * torch.maximum((x / scale).abs() * 2.0 ** -4, torch.tensor(2.0 ** -10, dtype=torch.float64, device=x.device))
+
+
+APPEND = [
+    # lens (with the new), rows, heads, kv heads, dim, page, rotated
+    ([1], [1], 4, 4, 64, 16, 64),
+    ([300], [1], 12, 12, 64, 32, 0),
+    ([1, 16, 17, 64, 65, 1000, 33], [1] * 7, 8, 2, 128, 16, 128),
+    ([700, 64, 5, 130, 40], [500, 64, 0, 3, 40], 8, 2, 128, 64, 64),
+    ([65, 100], [2, 37], 6, 2, 96, 64, 48),
+    ([40, 100], [15, 33], 5, 1, 80, 32, 2),
+    ([300], [290], 2, 2, 256, 64, 256),
+    ([70], [70], 3, 3, 2, 16, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens,rows,heads,kvh,dim,page,rot", APPEND)
+def test_append(lens, rows, heads, kvh, dim, page, rot, dtype):
+    before = [n - r for n, r in zip(lens, rows)]
+    cache = Cache(before, kvh, dim, page, 40 + sum(lens), spare=3 + sum(-(-n // page) for n in lens))
+    free = [p for p in range(cache.pool.shape[0]) if p not in set(cache.table.flatten().tolist())]
+    table = torch.full((len(lens), max(-(-n // page) for n in lens)), -1, dtype=torch.int32, device=DEV)
+    table[:, :cache.table.shape[1]] = cache.table[:, :table.shape[1]]
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            if table[b, i] < 0:
+                table[b, i] = free.pop()
+    cache.table = table
+    handle = pg.Kv8Cache(cache.pool, cache.scales, table, page_tokens=page, head_dim=dim)
+    total = sum(rows)
+    # rows of a product with more outputs than these: gaps between rows, odd addresses
+    wide = (torch.randn(total, (heads + 2 * kvh) * dim + 5, generator=gen(1), device=DEV) * 1.7).to(dtype)
+    qkv = wide[:, 1:1 + (heads + 2 * kvh) * dim].view(total, heads + 2 * kvh, dim)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kvh], qkv[:, heads + kvh:]
+    old_pool, old_scales, before_q = cache.pool.clone(), cache.scales.clone(), q.double()
+    old = [ref.sequence_kv(old_pool, old_scales, table[b], n, page, dim) for b, n in enumerate(before)]
+    one = all(r == 1 for r in rows)
+    handle.append(k, v, i32(lens), row_start=None if one else starts(rows), q=q, q_out=q, rot_dims=rot)
+    at, mine = 0, set()
+    for b, (n, length) in enumerate(zip(rows, lens)):
+        pos = torch.arange(length - n, length, device=DEV)
+        turned = ref.rotate(before_q[at:at + n], pos, rot, 10000.0)
+        got = qkv[at:at + n, :heads].double()
+        # turned in FP32: two products and a sum, then the type's rounding
+        assert ((got - turned).abs() <= U[dtype] * turned.abs() + 2.0 ** -22 * before_q[at:at + n].abs().amax(-1, keepdim=True)).all()
+        new = [ref.rotate(k[at:at + n].double(), pos, rot, 10000.0), v[at:at + n].double()]
+        held = ref.sequence_kv(cache.pool, cache.scales, table[b], length, page, dim)
+        for first in range((length - n) // page * page if n else length, length, page):
+            p, o, end = int(table[b, first // page]), max(length - n - first, 0), min(length - first, page)
+            mine.add(p)
+            for side in range(2):
+                part = new[side][first + o - (length - n):first + end - (length - n)]
+                for h in range(kvh):
+                    scale, amax = float(cache.scales[p, h, side]), float(part[:, h].abs().max())
+                    wants = {max(ref.block_scale(amax * f), float(old_scales[p, h, side]) if o else 0.0) for f in (1 - 1e-6, 1, 1 + 1e-6)}
+                    assert scale in wants, (b, first, side, h, scale, wants)
+                    x = held[side][first + o:first + end, h]
+                    assert ((x - part[:, h]).abs() <= quantised(part[:, h], scale) * (1 + 1e-6) + 1e-6 * amax).all()
+                    if o:  # earlier tokens: exact, or rounded once more where they became subnormal
+                        was, now = old[b][side][first:first + o, h], held[side][first:first + o, h]
+                        assert ((was - now).abs() <= (0.0 if scale == float(old_scales[p, h, side]) else scale * 2.0 ** -10)).all()
+        at += n
+    others = [p for p in range(cache.pool.shape[0]) if p not in mine]
+    assert torch.equal(cache.pool[others], old_pool[others])
+    assert torch.equal(cache.scales[others].view(torch.int32), old_scales[others].view(torch.int32))
+    # what lies behind the last token of a page is not touched
+    for b, length in enumerate(lens):
+        if rows[b] and length % page:
+            kb, vb = ref.blocks(cache.pool[table[b, length // page].long()], page, dim)
+            ko, vo = ref.blocks(old_pool[table[b, length // page].long()], page, dim)
+            assert torch.equal(kb[:, length % page:], ko[:, length % page:]) and torch.equal(vb[..., length % page:], vo[..., length % page:])
+
+
+def empty_cache(seqs, pages_per_seq, kvh, dim, page):
+    n = seqs * pages_per_seq
+    pool = torch.full(pg.Kv8Cache.pool_shape(n, kvh, page, dim), 255, dtype=torch.uint8, device=DEV)
+    scales = torch.full((n, kvh, 2), math.nan, device=DEV)
+    table = torch.randperm(n, device=DEV).to(torch.int32).view(seqs, pages_per_seq)
+    return pg.Kv8Cache(pool, scales, table, page_tokens=page, head_dim=dim)
+
+
+def test_append_token_by_token_is_append_at_once_up_to_subnormal_codes():
+    n, kvh, dim, page = 100, 2, 64, 32
+    g = gen(7)
+    k, v = (torch.randn(n, kvh, dim, generator=g, device=DEV) * torch.exp2(torch.rand(n, 1, 1, generator=g, device=DEV) * 6) for _ in range(2))
+    whole, single = empty_cache(1, 4, kvh, dim, page), empty_cache(1, 4, kvh, dim, page)
+    whole.append(k, v, i32([n]), row_start=i32([0, n]), rot_dims=dim)
+    for t in range(n):
+        single.append(k[t:t + 1], v[t:t + 1], i32([t + 1]), rot_dims=dim)
+    for i in range(4):
+        a, b = whole.scales[whole.page_table[0, i].long()], single.scales[single.page_table[0, i].long()]
+        assert torch.equal(a, b)
+    for x, y in zip(*(ref.sequence_kv(c.pool, c.scales, c.page_table[0], n, page, dim) for c in (whole, single))):
+        s = torch.stack([whole.scales[whole.page_table[0, t // page].long()] for t in range(n)]).amax(-1)[..., None]
+        # each growth of the scale rounds a subnormal code by at most half its step of 2^-9; the errors halve from growth to growth
+        assert ((x - y).abs() <= 2.0 ** -8 * s).all()
+        assert (x != y).float().mean() < 0.2
+
+
+def test_append_blocks_with_nan_or_infinity_and_zeros():
+    c = empty_cache(1, 3, 1, 64, 16)
+    k, v = torch.randn(40, 1, 64, device=DEV), torch.randn(40, 1, 64, device=DEV)
+    k[3, 0, 5], v[20, 0, 0] = math.nan, -math.inf
+    k[32:] = 0
+    v[33:] = 0
+    v[32] = 1e-38
+    c.append(k, v, i32([40]), row_start=i32([0, 40]))
+    s = c.scales[c.page_table[0].long()][:, 0]
+    assert torch.isnan(s[0, 0]) and torch.isfinite(s[0, 1]) and torch.isfinite(s[1, 0]) and torch.isnan(s[1, 1])
+    assert s[2, 0] == 2.0 ** -100 and s[2, 1] == 2.0 ** -100
+    q, out = torch.randn(1, 1, 64, device=DEV), torch.empty(1, 1, 64, device=DEV)
+    ws = torch.zeros(c.workspace_bytes(1, 1, F32), dtype=torch.uint8, device=DEV)
+    c.attention(q, out, i32([40]), ws)
+    assert torch.isnan(out).all()
+    c.attention(q, out, i32([40]), ws, window=8)  # the bad blocks are out of sight
+    assert torch.isfinite(out).all()
+    c.append(k[:1], v[:1], i32([21]))  # a page position in the middle: the block stays NaN
+    assert torch.isnan(c.scales[c.page_table[0, 1].long()][0, 1])
+    c.append(k[4:16], v[4:16], i32([12]), row_start=i32([0, 12]))  # the page anew
+    assert torch.isfinite(c.scales[c.page_table[0, 0].long()]).all()
+
+
+def test_append_rows_that_have_no_place():
+    c = empty_cache(3, 2, 1, 64, 16)
+    c.page_table[1, 0] = -1
+    c.page_table[1, 1] = 99
+    pool = c.pool.clone()
+    x = torch.randn(60, 1, 64, device=DEV)
+    # sequence 0: more rows than tokens, so its first rows lie before position 0; 1: no pages; 2: beyond its table
+    c.append(x, x, i32([3, 20, 40]), row_start=i32([0, 10, 30, 60]))
+    k, v = ref.sequence_kv(c.pool, c.scales, c.page_table[0], 3, 16, 64)
+    assert ((k - x[7:10].double()).abs() <= 0.07 * x[7:10].abs().double() + 1e-2).all()
+    assert ((v - x[7:10].double()).abs() <= 0.07 * x[7:10].abs().double() + 1e-2).all()
+    k, _ = ref.sequence_kv(c.pool, c.scales, c.page_table[2], 32, 16, 64)  # its rows 30..51 are positions 10..31
+    assert torch.isnan(k[10:16]).all()  # in a block that no append began, whose scale was NaN
+    assert ((k[16:] - x[36:52].double()).abs() <= 0.07 * x[36:52].abs().double() + 1e-2).all()
+    mine = set(c.page_table[[0, 2]].flatten().tolist()) - {int(c.page_table[0, 1])}
+    others = [p for p in range(6) if p not in mine]
+    assert torch.equal(c.pool[others], pool[others])
+
+
+# ------------------------------------------------------------------ 4-bit products
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,k,group", [(1, 1, 64), (16, 64, 64), (17, 65, 64), (33, 200, 128), (100, 129, 128), (48, 1024, 128), (5, 4096, 64)])
+def test_quantize_q4(n, k, group, dtype):
+    w = (torch.randn(n, k + 3, generator=gen(n + k), device=DEV) * torch.rand(n, 1, device=DEV)).to(dtype)[:, 1:k + 1]
+    w[0, :min(k, group)] = 0
+    ps, ss = pg.q4_shapes(n, k, group)
+    packed, scales = torch.full(ps, 77, dtype=torch.uint8, device=DEV), torch.full(ss, 3.0, dtype=BF16, device=DEV)
+    pg.quantize_q4(w, packed, scales, group)
+    x = torch.nn.functional.pad(w.float(), (0, ss[0] * group - k)).view(n, ss[0], group)
+    want = (x.abs().amax(-1) / 7).to(BF16)
+    assert torch.equal(scales[:, :n].t(), want) and (scales[:, n:] == 0).all()
+    s = want.float()[..., None]
+    code = torch.where(s > 0, torch.round(x / torch.where(s > 0, s, 1.0)), 0.0).clamp(-8, 7).view(n, -1)
+    full = ref.q4_codes(packed, ps[0] * 16, ps[1] * 64)
+    assert torch.equal(full[:n, :k].float() - 8, code[:, :k])
+    assert (full[n:] == 8).all() and (full[:, k:] == 8).all()
+
+
+LINEAR = [(1, 1, 1, 64), (1, 2304, 768, 64), (2, 17, 65, 64), (8, 100, 1600, 128), (9, 31, 200, 64), (16, 640, 4096, 128), (5, 4000, 300, 128), (3, 48, 16384, 64),
+          (16, 9000, 513, 64), (7, 33000, 70, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,n,k,group", LINEAR)
+def test_linear_q4(m, n, k, group, dtype):
+    g = gen(m + n + k)
+    ps, ss = pg.q4_shapes(n, k, group)
+    packed, scales = torch.empty(ps, dtype=torch.uint8, device=DEV), torch.empty(ss, dtype=BF16, device=DEV)
+    pg.quantize_q4(torch.randn(n, k, generator=g, device=DEV) * 0.05, packed, scales, group)
+    w = ref.q4_weights(packed, scales, n, k, group)
+    for gap, bias in ((0, True), (3, False)):  # rows with gaps are read value by value
+        x = torch.randn(m, k + gap, generator=g, device=DEV).to(dtype)[:, gap:]
+        b = torch.randn(n, generator=g, device=DEV).to(dtype) if bias else None
+        big = torch.full((m, n + 5), 9.0, device=DEV, dtype=dtype)
+        pg.linear_q4(x, packed, scales, big[:, 2:n + 2], group, bias=b)
+        want = x.double() @ w.t() + (b.double() if bias else 0.0)
+        size = x.double().abs() @ w.abs().t() + (b.double().abs() if bias else 0.0)
+        tile = x.double().abs().amax(-1, keepdim=True) * w.abs().sum(-1)  # a pair's rest is lost relative to the largest input of its tile
+        tol = 2.0 ** -18 * size + U[dtype] * want.abs() + (2.0 ** -21 * tile if dtype == F32 else 0.0)
+        assert ((big[:, 2:n + 2].double() - want).abs() <= tol).all()
+        assert (big[:, :2] == 9).all() and (big[:, n + 2:] == 9).all()
+
+
+def test_linear_q4_inputs_of_all_sizes():
+    n, k = 64, 256
+    ps, ss = pg.q4_shapes(n, k, 64)
+    packed, scales = torch.empty(ps, dtype=torch.uint8, device=DEV), torch.empty(ss, dtype=BF16, device=DEV)
+    pg.quantize_q4(torch.randn(n, k, generator=gen(1), device=DEV), packed, scales, 64)
+    w = ref.q4_weights(packed, scales, n, k, 64)
+    x = torch.randn(4, k, generator=gen(2), device=DEV)
+    x[0] *= 1e-30
+    x[1] *= 1e30
+    x[2, :64] *= 1e8  # tiles of one row that differ
+    x[3] = 0
+    out = torch.empty(4, n, device=DEV)
+    pg.linear_q4(x, packed, scales, out, 64)
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    assert ((out.double() - want).abs() <= 2.0 ** -18 * size).all()
+
+
+# ------------------------------------------------------------------ log probabilities
+def scores(x, targets, top):
+    """log p of targets, entropy, ids and log p of the top entries in float64, by the definition."""
+    x = x.double()
+    d = x - x.amax(-1, keepdim=True)  # values may be so large that the logarithm of their sum loses all but the maximum
+    p = d - torch.logsumexp(d, -1, keepdim=True)
+    lp = p.gather(1, targets.long().clamp(0, x.shape[1] - 1)[:, None])[:, 0]
+    ent = -(p.exp() * p.clamp(min=-1e30)).sum(-1)
+    ids = torch.argsort(-x, dim=-1, stable=True)[:, :top]
+    return lp, ent, ids, p.gather(1, ids)
+
+
+def run_scores(x, targets, top):
+    rows = x.shape[0]
+    lp, ent = torch.empty(rows, device=DEV), torch.empty(rows, device=DEV)
+    ids = torch.full((rows, top), -7, dtype=torch.int32, device=DEV) if top else None
+    values = torch.empty(rows, top, device=DEV) if top else None
+    pg.token_logprobs(x, targets, lp, ent, ids, values)
+    return lp, ent, ids, values
+
+
+def check_scores(x, targets, top):
+    got, want = run_scores(x, targets, top), scores(x, targets, top)
+    for a, b in ((got[0], want[0]), (got[1], want[1])) + (((got[3], want[3]),) if top else ()):
+        a = a.double()
+        same = (a == b) | ((a - b).abs() <= 2.0 ** -18 * (1 + b.abs()))
+        assert same.all(), (a[~same][:4], b[~same][:4])
+    if top:
+        assert torch.equal(got[2].long(), want[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (2, 7, 7), (3, 33, 32), (1, 50257, 5), (8, 50257, 20), (200, 1000, 1), (149, 5003, 32), (5, 128256, 8), (600, 2049, 0),
+                                            (1, 1000003, 32), (40, 40, 32)])
+def test_token_logprobs(rows, vocab, top, dtype):
+    g = gen(rows + vocab)
+    x = (torch.randn(rows, vocab + 3, generator=g, device=DEV) * 3).to(dtype)[:, 1:vocab + 1]  # rows at odd addresses
+    x[:, torch.randint(0, vocab, (vocab // 10,), generator=g, device=DEV)] = -math.inf
+    x[torch.isinf(x).all(-1)] = 0.5
+    targets = torch.randint(0, vocab, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    check_scores(x, targets, top)
+    check_scores(x.contiguous(), targets, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [5, 600, 50257])
+def test_token_logprobs_masks_and_ties(dtype, vocab):
+    """Ties go to the lower id, masked entries have no weight, rows of one kind of value work."""
+    low = torch.finfo(dtype).min
+    x = torch.zeros(10, vocab, device=DEV, dtype=dtype)  # row 0: all equal
+    x[1] = -math.inf
+    x[1, vocab - 2] = 3.0  # one entry
+    x[2] = low
+    x[2, 1] = -1.0
+    x[3] = low  # all at the lowest value: as good as equal
+    x[4] = torch.arange(vocab, device=DEV).to(dtype)  # rising: the last are the largest
+    x[5] = -torch.arange(vocab, device=DEV).to(dtype)
+    x[6, ::2] = -0.0  # equal to 0
+    x[7] = torch.where(torch.arange(vocab, device=DEV) % 3 == 0, 2.0, -math.inf)
+    x[8] = torch.finfo(dtype).max
+    x[9, -1] = 3e38
+    top = min(5, vocab)
+    t = torch.tensor([0, vocab - 2, 1, 2, vocab - 1, 0, 1, 0, 3, vocab - 1], dtype=torch.int32, device=DEV)
+    check_scores(x, t, top)
+
+
+def test_token_logprobs_rows_without_a_distribution_and_odd_targets():
+    for vocab in (9, 3000, 50257):
+        x = torch.randn(6, vocab, device=DEV)
+        x[1, vocab - 1] = math.nan
+        x[2, 0] = math.inf
+        x[3] = -math.inf
+        t = torch.tensor([-1, 0, 0, 0, vocab, -2], dtype=torch.int32, device=DEV)
+        lp, ent, ids, values = run_scores(x, t, 3)
+        assert lp[0] == 0 and torch.isnan(lp[1:]).all()
+        assert torch.isnan(ent[1:4]).all() and torch.isfinite(ent[[0, 4, 5]]).all()
+        assert (ids[1:4] == -1).all() and torch.isnan(values[1:4]).all() and (ids[[0, 4, 5]] >= 0).all()
+
+
+def test_token_logprobs_each_output_alone():
+    x = torch.randn(3, 777, device=DEV)
+    t = i32([5, 6, 776])
+    want = scores(x, t, 4)
+    lp, ent = torch.empty(3, device=DEV), torch.empty(3, device=DEV)
+    pg.token_logprobs(x, targets=t, logprobs=lp)
+    pg.token_logprobs(x, entropy=ent)
+    ids, values = torch.empty(3, 4, dtype=torch.int32, device=DEV), torch.empty(3, 4, device=DEV)
+    pg.token_logprobs(x, top_ids=ids, top_logprobs=values)
+    assert ((lp - want[0]).abs() < 1e-4).all() and ((ent - want[1]).abs() < 1e-4).all()
+    assert torch.equal(ids.long(), want[2])
+
+
+# ------------------------------------------------------------------ together
+class Layer:
+    """One layer's step as a serving program builds it from the operators: products in 4 bits around the 8-bit cache, then a head."""
+
+    def __init__(self, dtype, seqs, heads=8, kvh=2, dim=64, vocab=1000, page=16, pages=8):
+        g = gen(5)
+        self.dtype, self.heads, self.kvh, self.dim, self.width = dtype, heads, kvh, dim, heads * dim
+        self.cache = empty_cache(seqs, pages, kvh, dim, page)
+        self.weights = {}
+        for name, n, k in (("qkv", (heads + 2 * kvh) * dim, self.width), ("o", self.width, self.width), ("head", vocab, self.width)):
+            ps, ss = pg.q4_shapes(n, k, 64)
+            packed, scales = torch.empty(ps, dtype=torch.uint8, device=DEV), torch.empty(ss, dtype=BF16, device=DEV)
+            pg.quantize_q4(torch.randn(n, k, generator=g, device=DEV) * k ** -0.5, packed, scales, 64)
+            self.weights[name] = packed, scales
+        e = lambda *s, t=dtype: torch.empty(*s, dtype=t, device=DEV)
+        self.x, self.lens = e(seqs, self.width), torch.zeros(seqs, dtype=torch.int32, device=DEV)
+        self.qkv, self.attn, self.y, self.logits = e(seqs, (heads + 2 * kvh) * dim), e(seqs, heads, dim), e(seqs, self.width), e(seqs, vocab)
+        self.ids, self.values, self.ent = e(seqs, 4, t=torch.int32), e(seqs, 4, t=F32), e(seqs, t=F32)
+        self.ws = torch.zeros(self.cache.workspace_bytes(seqs, heads, dtype), dtype=torch.uint8, device=DEV)
+
+    def step(self):
+        s = torch.cuda.current_stream().cuda_stream
+        h, kvh = self.heads, self.kvh
+        pg.linear_q4(self.x, *self.weights["qkv"], self.qkv, 64, stream=s)
+        rows = self.qkv.view(-1, h + 2 * kvh, self.dim)
+        q, k, v = rows[:, :h], rows[:, h:h + kvh], rows[:, h + kvh:]
+        self.cache.append(k, v, self.lens, q=q, q_out=q, rot_dims=self.dim, stream=s)
+        self.cache.attention(q, self.attn, self.lens, self.ws, stream=s)
+        pg.linear_q4(self.attn.view(-1, self.width), *self.weights["o"], self.y, 64, stream=s)
+        pg.linear_q4(self.y, *self.weights["head"], self.logits, 64, stream=s)
+        pg.token_logprobs(self.logits, entropy=self.ent, top_ids=self.ids, top_logprobs=self.values, stream=s)
+
+    def weight(self, name, n):
+        return ref.q4_weights(*self.weights[name], n, self.width, 64)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_step_of_all_operators_eager_and_captured(dtype):
+    seqs = 5
+    eager, captured = Layer(dtype, seqs), Layer(dtype, seqs)
+    captured.cache.page_table.copy_(eager.cache.page_table)
+    for l in (eager, captured):  # different lengths to begin with
+        l.lens.copy_(torch.arange(seqs))
+    stream = torch.cuda.Stream()
+    captured.x.zero_()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        captured.step()
+    inputs = torch.randn(60, seqs, eager.width, generator=gen(8), device=DEV).to(dtype)
+    # both caches start with the same tokens at the positions before the first step
+    for l in (eager, captured):
+        kv = torch.randn(int(sum(range(seqs))), 2, 64, generator=gen(9), device=DEV).to(dtype)
+        l.cache.append(kv, kv, l.lens, row_start=starts(list(range(seqs))))
+    history = [[] for _ in range(seqs)]
+    for t in range(60):
+        for l in (eager, captured):
+            l.x.copy_(inputs[t])
+            l.lens.add_(1)
+        eager.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in ("qkv", "attn", "y", "logits", "ids", "values", "ent"):
+            assert torch.equal(getattr(eager, name), getattr(captured, name)), (t, name)
+        if t not in (0, 20, 59):
+            continue
+        # each operator against its definition, from what the one before it gave
+        n = eager.qkv.shape[1]
+        raw = eager.x.double() @ eager.weight("qkv", n).t()
+        size = eager.x.double().abs() @ eager.weight("qkv", n).abs().t()
+        v = eager.qkv.view(seqs, -1, 64)[:, 10:].double()
+        assert ((v.flatten(1) - raw[:, 640:]).abs() <= 2.0 ** -17 * size[:, 640:] + U[dtype] * raw[:, 640:].abs()).all()
+        for b in range(seqs):
+            length = int(eager.lens[b])
+            keys, values = ref.sequence_kv(eager.cache.pool, eager.cache.scales, eager.cache.page_table[b], length, 16, 64)
+            want = ref.attention(eager.qkv.view(seqs, -1, 64)[b:b + 1, :8].double(), keys, values, torch.tensor([length - 1], device=DEV), 0.125)
+            tol = values.abs().max() * (2.0 ** -15 if dtype == F32 else 2.0 ** -10) + U[dtype] * want.abs()
+            assert ((eager.attn[b:b + 1].double() - want).abs() <= tol).all()
+        want = scores(eager.logits, torch.zeros(seqs, device=DEV), 4)
+        assert torch.equal(eager.ids.long(), want[2]) and ((eager.ent - want[1]).abs() <= 2.0 ** -16 * (1 + want[1])).all()
+
+
+def test_two_streams_at_once():
+    """Calls that overlap, each with a workspace of its own, give what they give alone."""
+    a, b = Cache([9000, 40], 2, 64, 64, 1), Cache([8000, 50], 2, 64, 64, 2)
+    qs = [torch.randn(2, 8, 64, generator=gen(i), device=DEV) for i in range(2)]
+    alone, both = [], [torch.empty_like(q) for q in qs]
+    spaces = [workspace(c, 2, 8, F32) for c in (a, b)]
+    lens = [i32(c.lens) for c in (a, b)]
+    for c, q, l, w in zip((a, b), qs, lens, spaces):
+        out = torch.empty_like(q)
+        c.handle.attention(q, out, l, w)
+        alone.append(out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, q, l, w, o, s in zip((a, b), qs, lens, spaces, both, streams):
+            c.handle.attention(q, o, l, w, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(alone, both))
