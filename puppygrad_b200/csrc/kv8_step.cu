@@ -1,21 +1,24 @@
 // Attention over the 8-bit paged cache for few rows of a sequence (a step's single token, several guesses of one).
 //
-// Work: a tile is up to 16 (FP32: 8) rows that share a key / value head, i.e. (token, query head of the group) pairs; a unit is a tile
-// times 64 consecutive positions. All units of a call, in the order sequence, head, tile, position, are cut into equal contiguous
-// shares, one for each CTA of a persistent grid, and a CTA's into one for each warp: every SM reads the same number of bytes whatever
-// the lengths are. A tile that several warps share is put together in shared memory, one that several CTAs share by the CTA that
-// arrives last, in the order of the positions (the result does not hang on who that is).
+// Work: a tile is 8 or 16 rows that share a key / value head, i.e. (token, query head of the group) pairs; a unit is a tile times 64
+// consecutive positions. All units of a call, in the order sequence, head, tile, position, are cut into equal contiguous shares,
+// one for each CTA of a persistent grid, and a CTA's into one for each warp: every SM reads the same number of bytes whatever the
+// lengths are. Parts of a tile that several warps share are merged by their CTA, those of several CTAs by the one that arrives
+// last, in the order of the positions (the result does not hang on who that is).
 //
-// A unit: S = Q K^T and O += P V by m16n8k16 FP16 matrix instructions, codes turned into FP16 (exact) in registers. The k index of a
-// product may be permuted as long as both operands agree, so a lane takes 16 consecutive bytes of a key row (4 k steps) and 16
-// consecutive tokens of a value row (values lie by head entry), and column n of score tile j stands for token 16 (n / 2) + 2 j +
-// (n & 1): a lane's probabilities are then those of the tokens whose values it holds, and no data passes between lanes.
+// A unit: S^T = K Q^T and O^T += V^T P^T by m16n8k16 FP16 matrix instructions: 16 tokens (or head entries) as rows, 8 of the tile's
+// rows as columns, codes turned into FP16 (exact) in registers. With the tokens as rows, a tile of 8 wastes nothing and costs half the
+// instructions and accumulators of the other order. The k index of a product may be permuted as long as both operands agree: a
+// lane takes 16 consecutive bytes of a key (4 k steps) and 16 consecutive tokens of a value row (values lie by head entry). Row r of
+// score tile s is token 16 ((r % 8) / 2) + 4 s + 2 (r / 8) + r % 2, so that a transposition of 8x8 blocks (movmatrix) makes the
+// weights the operand that goes with the values a lane holds.
 //
 // Softmax with the blocks' scales: the key scale multiplies the score, the value scale is part of the exponent, w = 2^(s log2 e +
 // log2 scale_v - m), so that O = sum w code and the weights stay within [0, 1] however the scales differ; the denominator adds w /
-// scale_v. m is the running maximum of that exponent. FP32 queries: rows 0..7 of the instruction's tile hold the FP16 parts hi of
-// q and of the weights, rows 8..15 the rests lo, their sums are added afterwards: FP32 grade at the price of one instruction.
-// Rounding: BF16 queries are exact in FP16 after the row's scaling to [1, 2), their weights round to FP16 (2^-12 of the largest).
+// scale_v. m is the running maximum of that exponent. FP32 queries and their weights are pairs of FP16 numbers, two instructions
+// into one accumulator: FP32 grade. Rounding: BF16 queries are exact in FP16 after their row's scaling to [1, 2), their weights round
+// to FP16 (2^-12 of the largest).
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -25,10 +28,16 @@ namespace {
 
 constexpr int UNIT = 64;  // positions
 
-template <int DP>
+// Bytes come through a ring of slots for every warp, 64 tokens times 64 head entries (4 KB) each, keys of a unit first, then its
+// values: all but one are on their way while that one is worked on, 128 KB for an SM.
+template <int DP, int NB>
 struct Shape {
-  static constexpr int WARPS = DP <= 128 ? 8 : 4;  // partial tiles of all warps fit shared memory
+  static constexpr int KC = DP / 64;                                    // key slots (and value slots) of a unit
+  static constexpr int WARPS = DP == 64 || (DP == 128 && NB == 1) ? 16 : 8;  // by registers
   static constexpr int THREADS = WARPS * 32;
+  static constexpr int SLOT = 4096, SLOTS = WARPS == 16 ? 3 : 2 * KC + 1 < 6 ? 2 * KC + 1 : 6, AHEAD = SLOTS - 1;
+  static constexpr int ROWS = 8 * NB, PART = ROWS * (DP + 2);
+  static constexpr int SMEM = WARPS * SLOTS * SLOT;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -40,11 +49,17 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {  // an 8x8 block of FP16
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 // Pieces of 64 positions that any row of a sequence sees: [0, keep) and [low, high).
@@ -61,441 +76,618 @@ __device__ __forceinline__ Span span_of(const Kv8AttnArgs& a, int len, int n) {
   return s;
 }
 
-template <int DP, typename T>
-__global__ void __launch_bounds__(Shape<DP>::THREADS) kv8_step_kernel(Kv8AttnArgs a) {
+// 16 bytes from global to shared memory, asynchronously; zeros where `live` is false (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 shared16(uint32_t from) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+  return v;
+}
+// 16 consecutive values of a row, zeros from `dim` on (and where there is no row).
+template <typename T>
+struct Sixteen {
+  uint4 w[sizeof(T)];
+  __device__ __forceinline__ void load(const T* q, int d, int dim, bool wide) {
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); ++i) {
+        constexpr int N = 16 / sizeof(T);
+        w[i] = q && d + (i + 1) * N <= dim ? *reinterpret_cast<const uint4*>(q + d + i * N) : make_uint4(0, 0, 0, 0);
+      }
+    } else {
+      union {
+        uint4 u[sizeof(T)];
+        T t[16];
+      } x;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x.t[e] = q && d + e < dim ? q[d + e] : from_f32<T>(0.f);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); ++i) w[i] = x.u[i];
+    }
+  }
+  __device__ __forceinline__ float2 two(int i) const {  // values 2 i and 2 i + 1
+    const uint32_t r[4] = {w[i / (8 / sizeof(T))].x, w[i / (8 / sizeof(T))].y, w[i / (8 / sizeof(T))].z, w[i / (8 / sizeof(T))].w};
+    if (sizeof(T) == 4) return make_float2(__uint_as_float(r[2 * (i & 1)]), __uint_as_float(r[2 * (i & 1) + 1]));
+    return make_float2(__uint_as_float(r[i & 3] << 16), __uint_as_float(r[i & 3] & 0xFFFF0000u));
+  }
+};
+
+// A tile of rows, and where its units lie among all units.
+struct Tile {
+  int b, head, row0, rows, first_row, n_rows, len, have, first_unit, units, counter;
+  Span span;
+};
+// Equal shares of the units: share i begins at floor(i * units / n), without 64-bit divisions. Shares of equal tiles begin where
+// tiles do if n is a multiple of their number.
+struct Shares {
+  int units, n, each, more;
+  __device__ __forceinline__ Shares(int u, int k) : units(u), n(k), each(u / k), more(u - u / k * k) {}
+  __device__ __forceinline__ int begin(int i) const { return i * each + i * more / n; }
+  __device__ __forceinline__ int of(int u) const {
+    int i = min((int)(((float)u + 0.5f) / (float)units * (float)n), n - 1);
+#pragma unroll 1
+    while (begin(i) > u) --i;
+#pragma unroll 1
+    while (i + 1 < n && begin(i + 1) <= u) ++i;
+    return i;
+  }
+};
+
+template <int DP, typename T, int NB>
+__global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8AttnArgs a) {
   constexpr bool PAIR = std::is_same<T, float>::value;
-  constexpr int WARPS = Shape<DP>::WARPS, THREADS = Shape<DP>::THREADS, ROWS = PAIR ? 8 : 16, PART = ROWS * (DP + 2);
-  constexpr int KC = DP / 64, NT = DP / 8;
+  using S = Shape<DP, NB>;
+  constexpr int WARPS = S::WARPS, THREADS = S::THREADS, ROWS = S::ROWS, PART = S::PART, KC = S::KC, SLOT = S::SLOT, AHEAD = S::AHEAD, MT = DP / 16;
+  static_assert(PART * 4 <= S::SLOTS * SLOT, "a warp's last part takes the place of its ring");
+  static_assert(AHEAD <= 2 * KC, "the ring reaches into the next unit at most");
   extern __shared__ __align__(16) uint8_t smem[];
-  // [WARPS][DP / 16][32] uint4 queries, [WARPS][2][PART] floats, then the units' and the counters' prefix of the sequences
-  uint4* qf = reinterpret_cast<uint4*>(smem) + (threadIdx.x >> 5) * (DP / 16) * 32;
-  float* parts = reinterpret_cast<float*>(smem + WARPS * (DP / 16) * 512);
-  int* unit_end = reinterpret_cast<int*>(parts + WARPS * 2 * PART);
-  __shared__ int scan[Shape<DP>::THREADS];
-  __shared__ int part_tile[WARPS * 2];  // counter of the tile that a partial belongs to, -1: none
+  __shared__ int scan[THREADS];  // units of the sequences up to thread t's last
+  __shared__ int wsum[WARPS];
+  __shared__ int part_tile[WARPS * 2];  // first unit of the tile that a part belongs to, -1: none
+  __shared__ Tile part_of_tile[WARPS * 2];
+  __shared__ float factor[ROWS][KV8_MAX_CTAS], row_max[ROWS], row_sum[ROWS];
   __shared__ int last_here;
 
   const Kv8View& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::SLOTS * SLOT) + lane * 16;  // this lane's 16 bytes of every 512
+  // parts: a warp's last one in its ring, one before it (of another tile) in global memory
+  auto last_part = [&](int w) { return reinterpret_cast<float*>(smem + w * S::SLOTS * SLOT); };
+  float* const warp_parts = a.partials + (size_t)gridDim.x * 2 * PART;
+  auto early_part = [&](int w) { return warp_parts + ((size_t)blockIdx.x * WARPS + w) * PART; };
 
-  auto tiles_of = [&](const SeqRows& r) { return (r.n * a.group + ROWS - 1) / ROWS; };
-  // ---- units of every sequence, summed up
+  // ---- units of every sequence, summed up: thread t has sequences per * t and following
+  auto tiles_of = [&](int n) { return (n * a.group + ROWS - 1) / ROWS; };
+  auto units_of = [&](int b) {
+    const int n = seq_rows(a.row_start, a.rows, b).n;
+    return n && (int64_t)n * a.group <= a.step_rows ? tiles_of(n) * c.kv_heads * span_of(a, max(a.lens[b], 0), n).units() : 0;
+  };
+  grid_dep_launch();
+  grid_dep_wait();
+  // the page table will be asked for as soon as the lengths are known
+#pragma unroll 1
+  for (int64_t i = (int64_t)tid * 32; i < (int64_t)c.seqs * c.pages_per_seq && i < THREADS * 32; i += THREADS * 32)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(c.table + i));
+  const int per = c.seqs <= THREADS ? 1 : (c.seqs + THREADS - 1) / THREADS;
   {
-    const int per = (c.seqs + THREADS - 1) / THREADS, b0 = min(tid * per, c.seqs), b1 = min(b0 + per, c.seqs);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      const SeqRows r = seq_rows(a.row_start, a.rows, b);
-      if (r.n) sum += tiles_of(r) * c.kv_heads * span_of(a, max(a.lens[b], 0), r.n).units();
-      unit_end[b] = sum;
+#pragma unroll 1
+    for (int b = tid * per; b < min(tid * per + per, c.seqs); ++b) sum += units_of(b);
+    int up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(ALL_LANES, up, o);
+      if (lane >= o) up += v;
     }
-    scan[tid] = sum;
-    __syncthreads();
-    for (int o = 1; o < THREADS; o <<= 1) {
-      const int v = tid >= o ? scan[tid - o] : 0;
-      __syncthreads();
-      scan[tid] += v;
-      __syncthreads();
-    }
-    const int before = tid ? scan[tid - 1] : 0;
-    for (int b = b0; b < b1; ++b) unit_end[b] += before;
+    if (lane == 31) wsum[warp] = up;
+    scan[tid] = up;
     if (tid < WARPS * 2) part_tile[tid] = -1;
     __syncthreads();
   }
-  const int units = unit_end[c.seqs - 1];
-  const int ctas = min((int)gridDim.x, units);
+  int total = lane < WARPS ? wsum[lane] : 0;  // lane i: units up to those of warp i's threads
+#pragma unroll
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const int v = __shfl_up_sync(ALL_LANES, total, o);
+    if (lane >= o) total += v;
+  }
+  const int units = __shfl_sync(ALL_LANES, total, WARPS - 1);
+  if (units == 0) return;
+  // no more CTAs than give each warp a unit; for a single sequence a number that lets CTAs begin where tiles do
+  int ctas = min((int)gridDim.x, (units + WARPS - 1) / WARPS);
+  if (c.seqs == 1) {
+    const int tiles = tiles_of(seq_rows(a.row_start, a.rows, 0).n) * c.kv_heads;
+    if (tiles <= (int)gridDim.x) ctas = min((int)gridDim.x / tiles, (units / tiles + WARPS - 1) / WARPS) * tiles;
+  }
   if ((int)blockIdx.x >= ctas) return;
-  auto cta_begin = [&](int i) { return (int)((int64_t)units * i / ctas); };
-  const int c0 = cta_begin(blockIdx.x), c1 = cta_begin(blockIdx.x + 1);
-  const int u0 = c0 + (int)((int64_t)(c1 - c0) * warp / WARPS), u1 = c0 + (int)((int64_t)(c1 - c0) * (warp + 1) / WARPS);
+  const Shares shares(units, ctas);
+  const int c0 = shares.begin(blockIdx.x), c1 = shares.begin(blockIdx.x + 1);
+  const int u0 = c0 + (c1 - c0) * warp / WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / WARPS;
 
-  // writes one row of a finished tile: `value(d)` is the sum of weighted codes, `l` the denominator
+  auto tile_at = [&](int u) {  // by the whole warp
+    const int w = __ffs(__ballot_sync(ALL_LANES, lane < WARPS && total > u)) - 1;
+    int before = w ? __shfl_sync(ALL_LANES, total, w - 1) : 0;
+    const int up = scan[w * 32 + lane];
+    const int i = __ffs(__ballot_sync(ALL_LANES, before + up > u)) - 1;
+    if (i) before += __shfl_sync(ALL_LANES, up, i - 1);
+    Tile t;
+    t.b = (w * 32 + i) * per;
+#pragma unroll 1
+    for (int k = 1; k < per; ++k) {
+      const int n = units_of(t.b);
+      if (before + n > u) break;
+      before += n;
+      ++t.b;
+    }
+    const SeqRows r = seq_rows(a.row_start, a.rows, t.b);
+    t.first_row = r.first;
+    t.n_rows = r.n;
+    t.len = max(a.lens[t.b], 0);
+    t.have = min(t.len, c.pages_per_seq << c.page_shift);
+    t.span = span_of(a, t.len, r.n);
+    t.units = t.span.units();
+    const int tiles = tiles_of(r.n), x = (u - before) / t.units;
+    t.first_unit = before + x * t.units;
+    t.head = tiles == 1 ? x : x / tiles;
+    const int tile = x - t.head * tiles;
+    t.row0 = tile * ROWS;
+    t.rows = min(ROWS, r.n * a.group - t.row0);
+    t.counter = ((int)((int64_t)r.first * a.group / ROWS) + t.b + tile) * c.kv_heads + t.head;
+    return t;
+  };
+  auto start_of = [&](const Span& s, int x) { return (x < s.keep ? x : s.low + x - s.keep) * UNIT; };
+
+  const size_t block = (size_t)DP << c.page_shift;
+#pragma unroll 1
   for (int u = u0; u < u1;) {
-    // ---- the tile of unit u
-    int lo = 0, hi = c.seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (unit_end[mid] > u) hi = mid;
-      else lo = mid + 1;
-    }
-    const int b = lo;
-    const SeqRows r = seq_rows(a.row_start, a.rows, b);
-    const int len = max(a.lens[b], 0), have = min(len, c.pages_per_seq << c.page_shift);
-    const Span span = span_of(a, len, r.n);
-    const int n = span.units(), tiles = tiles_of(r);
-    const int in_seq = u - (b ? unit_end[b - 1] : 0), tile_i = in_seq / n, x0 = in_seq - tile_i * n;
-    const int head = tile_i / tiles, tile = tile_i - head * tiles;
-    const int x1 = min(n, x0 + (u1 - u));
-    const int row0 = tile * ROWS, rows = min(ROWS, r.n * a.group - row0);  // in (token, head of the group) pairs
-    // positions of this lane's rows g and g + 8 (FP32: both halves are row g)
-    auto pos_of = [&](int i) { return len - r.n + (row0 + min(i, rows - 1)) / a.group; };
-    const int pos_a = pos_of(g), pos_b = PAIR ? pos_a : pos_of(g + 8);
-    const int pos_low = pos_of(0), pos_high = pos_of(rows - 1);
-
-    // ---- queries into fragments, each row scaled by a power of two to [1, 2)
-    float fa, fb;  // what brings a row's product back, times scale log2 e
-    {
-      auto query = [&](int i) -> const T* {
-        const int x = row0 + i, t = x / a.group;
-        return (const T*)a.q + (size_t)(r.first + t) * a.q_row + (size_t)(head * a.group + (x - t * a.group)) * c.dim;
-      };
-      const T* qa = g < rows ? query(g) : nullptr;
-      const T* qb = !PAIR && g + 8 < rows ? query(g + 8) : nullptr;
-      auto at = [&](const T* q, int d) { return q && d < c.dim ? to_f32(q[d]) : 0.f; };
-      float ma = 0.f, mb = 0.f;
-      for (int d = cc; d < c.dim; d += 4) {
-        ma = fmaxf(ma, fabsf(at(qa, d)));
-        mb = fmaxf(mb, fabsf(at(qb, d)));
-      }
+    const Tile t = tile_at(u);
+    const int x0 = u - t.first_unit, x1 = min(t.units, x0 + (u1 - u));
+    // ---- fetching runs AHEAD slots in front of computing, and the look-up of a unit's pages a unit in front of that
+    struct Source {
+      const uint8_t *k, *v;  // of this lane's first 16 bytes
+      bool k_live, v_live;
+      int page;      // of this lane's scores: tokens 16 (g / 2) and following
+      float2 scale;  // of that page: keys, values
+    };
+    int fx = x0, f_page = -1;  // next unit to fetch, its page
+    auto look_up = [&] {
+      const int tok = start_of(t.span, fx) + (g >> 1) * 16;
+      f_page = fx < x1 && tok < t.have ? c.table[(size_t)t.b * c.pages_per_seq + (tok >> c.page_shift)] : -1;
+    };
+    auto next_source = [&](Source& s) {
+      const int f_t0 = start_of(t.span, fx), mask = c.page_tokens - 1;
+      s.page = (unsigned)f_page < (unsigned)c.n_pages ? f_page : -1;
+      const int page_v = __shfl_sync(ALL_LANES, s.page, cc * 8);  // of the values: tokens 16 cc and following
+      s.k = c.pool + ((size_t)max(s.page, 0) * c.kv_heads + t.head) * 2 * block + (size_t)(((f_t0 + (g >> 1) * 16) & mask) + (g & 1)) * DP + cc * 16;
+      s.v = c.pool + (((size_t)max(page_v, 0) * c.kv_heads + t.head) * 2 + 1) * block + ((f_t0 + cc * 16) & mask) + ((size_t)g << c.page_shift);
+      s.k_live = s.page >= 0;
+      s.v_live = page_v >= 0;
+      s.scale = make_float2(0.f, 1.f);
+      if (s.k_live) s.scale = *reinterpret_cast<const float2*>(c.scales + ((size_t)s.page * c.kv_heads + t.head) * 2);
+      ++fx;
+      look_up();
+    };
+    int wr = 0, rd = 0;  // ring positions, in bytes
+    auto fetch = [&](const Source& s, int i) {  // slot i of a unit
+      const uint32_t to = ring + wr;
+      wr = wr == (S::SLOTS - 1) * SLOT ? 0 : wr + SLOT;
+      if (i < KC) {
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        ma = fmaxf(ma, __shfl_xor_sync(ALL_LANES, ma, o));
-        mb = fmaxf(mb, __shfl_xor_sync(ALL_LANES, mb, o));
+        for (int j = 0; j < 8; ++j) copy16(to + j * 512, s.k + 2 * j * DP + i * 64, s.k_live);
+      } else {
+        const uint8_t* from = s.v + ((size_t)((i - KC) * 64) << c.page_shift);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) copy16(to + j * 512, from + ((j * 8) << c.page_shift), s.v_live);
       }
+    };
+    Source cur, nxt;
+    look_up();
+    next_source(cur);
+    nxt = cur;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      fetch(cur, i);
+      copy_commit();
+    }
+    // ---- queries: lane (g, cc) takes row g; behind the first keys and values, which take longer
+    const bool wide = (((uintptr_t)a.q | (uintptr_t)(a.q_row * sizeof(T)) | (uintptr_t)(c.dim * sizeof(T))) & 15) == 0;
+    Sixteen<T> raw[NB][KC];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int x = t.row0 + n * 8 + g, r = t.n_rows == 1 ? 0 : x / a.group;
+      const T* q = n * 8 + g < t.rows ? (const T*)a.q + (size_t)(t.first_row + r) * a.q_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim : nullptr;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) raw[n][i].load(q, i * 64 + cc * 16, c.dim, wide);
+    }
+    auto pos_of = [&](int i) { return t.n_rows == 1 ? t.len - 1 : t.len - t.n_rows + (t.row0 + min(i, t.rows - 1)) / a.group; };
+    const int pos_low = pos_of(0), pos_high = pos_of(t.rows - 1);
+    int pos[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) pos[n][e] = pos_of(n * 8 + cc * 2 + e);
+
+    // ---- queries as the column operand, each row scaled by a power of two to [1, 2)
+    uint32_t qh[NB][MT][2], ql[PAIR ? NB : 1][PAIR ? MT : 1][2];
+    float back[NB][2];  // what brings the products of rows 2 cc and 2 cc + 1 back, times scale log2 e
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 v = raw[n][i].two(e);
+          m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
+      m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 2));
       // exponents within +-100 keep both the factor and its inverse normal numbers
-      auto exponent = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100); };
-      const int ea = exponent(ma), eb = exponent(mb);
-      const float sa = __uint_as_float((uint32_t)(127 - ea) << 23), sb = __uint_as_float((uint32_t)(127 - eb) << 23);
-      fa = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ea) << 23);
-      fb = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + eb) << 23);
-      for (int i = 0; i < DP / 16; ++i) {
-        const int d = (i >> 2) * 64 + cc * 16 + (i & 3) * 4;
-        float v[4];
+      const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
+      const float f = __uint_as_float((uint32_t)(127 - ex) << 23);
+      const float b = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23);
+      back[n][0] = __shfl_sync(ALL_LANES, b, cc * 8);
+      back[n][1] = __shfl_sync(ALL_LANES, b, cc * 8 + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = at(qa, d + e) * sa;
-        uint4 f;
-        f.x = pack_f16(v[0], v[1]);
-        f.z = pack_f16(v[2], v[3]);
-        if (PAIR) {
-          const float2 p = __half22float2(*reinterpret_cast<__half2*>(&f.x)), q = __half22float2(*reinterpret_cast<__half2*>(&f.z));
-          f.y = pack_f16(v[0] - p.x, v[1] - p.y);
-          f.w = pack_f16(v[2] - q.x, v[3] - q.y);
-        } else {
-          f.y = pack_f16(at(qb, d) * sb, at(qb, d + 1) * sb);
-          f.w = pack_f16(at(qb, d + 2) * sb, at(qb, d + 3) * sb);
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 v = raw[n][i].two(e);
+          const uint32_t h = pack_f16(v.x * f, v.y * f);
+          qh[n][i * 4 + e / 2][e & 1] = h;
+          if constexpr (PAIR) {
+            const float2 r = unpack_f16(h);
+            ql[n][i * 4 + e / 2][e & 1] = pack_f16(v.x * f - r.x, v.y * f - r.y);
+          }
         }
-        qf[i * 32 + lane] = f;
-      }
-      __syncwarp();
     }
 
-    float o[NT][4];
+      float o[MT][NB][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+      float m[NB][2], l[NB][2];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
 
-    for (int x = x0; x < x1; ++x) {
-      const int t0 = (x < span.keep ? x : span.low + x - span.keep) * UNIT;
-      if (t0 > pos_high) break;  // later pieces are later positions: none of the tile's rows sees them
-      // this lane's 16 tokens: their page and scales
-      const int tok = t0 + cc * 16;
-      const int page = tok < have ? page_of(c, b, tok >> c.page_shift) : -1;
-      float ks = 0.f, ev = 0.f, inv_v = 1.f;
-      if (page >= 0) {
-        const float2 s = *reinterpret_cast<const float2*>(c.scales + ((size_t)page * c.kv_heads + head) * 2);
-        ks = s.x;
-        ev = __log2f(fmaxf(s.y, 7.888609e-31f));  // 2^-100, the least scale that an append writes
-        inv_v = 1.f / fmaxf(s.y, 7.888609e-31f);
-        if (s.y != s.y) ev = s.y, inv_v = 1.f;
-      }
-      const size_t block = (size_t)(DP << c.page_shift);
-      const int page_k = __shfl_sync(ALL_LANES, page, g >> 1);  // of the keys that this lane loads: chunk g / 2
-      const int off_k = ((t0 + (g >> 1) * 16) & (c.page_tokens - 1)) + (g & 1);
-      const uint8_t* kp = c.pool + ((size_t)max(page_k, 0) * c.kv_heads + head) * 2 * block + (size_t)off_k * DP + cc * 16;
-      const uint8_t* vp = c.pool + (((size_t)max(page, 0) * c.kv_heads + head) * 2 + 1) * block + (tok & (c.page_tokens - 1)) + ((size_t)g << c.page_shift);
-
-      float s[8][4];
+#pragma unroll 1
+      for (int x = x0; x < x1; ++x, ++u) {
+        const int t0 = start_of(t.span, x), tok = t0 + (g >> 1) * 16 + (g & 1);  // this lane's scores: tok + 2 j, j = 0..7
+        // waits for slot i, has the one AHEAD of it sent for, and gives its place
+        auto slot = [&](int i) {
+          copy_wait<AHEAD - 1>();
+          const uint32_t from = ring + rd;
+          rd = rd == (S::SLOTS - 1) * SLOT ? 0 : rd + SLOT;
+          const int k = i + AHEAD;
+          if (k < 2 * KC) {
+            fetch(cur, k);
+          } else {
+            if (x + 1 < x1) {
+              if (k == 2 * KC) next_source(nxt);
+              fetch(nxt, k - 2 * KC);
+            }
+          }
+          copy_commit();
+          return from;
+        };
+        float s[4][NB][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+          for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        uint4 kv[8];
+            for (int e = 0; e < 4; ++e) s[j][n][e] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) kv[j] = __ldg(reinterpret_cast<const uint4*>(kp + (size_t)2 * j * DP + i * 64));
-        uint4 q[4];
+        for (int i = 0; i < KC; ++i) {
+          const uint32_t from = slot(i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = qf[(i * 4 + e) * 32 + lane];
+          for (int j = 0; j < 4; ++j) {  // tokens of rows r and r + 8: key rows 2 j and 2 j + 1 of the lane
+            const uint4 k0 = shared16(from + 2 * j * 512), k1 = shared16(from + (2 * j + 1) * 512);
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t w[4] = {kv[j].x, kv[j].y, kv[j].z, kv[j].w};
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t f0 = e4m3x2_to_f16x2(w0[e] & 0xFFFFu), f1 = e4m3x2_to_f16x2(w1[e] & 0xFFFFu), f2 = e4m3x2_to_f16x2(w0[e] >> 16),
+                             f3 = e4m3x2_to_f16x2(w1[e] >> 16);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mma_f16(s[j], q[e].x, q[e].y, q[e].z, q[e].w, e4m3x2_to_f16x2(w[e] & 0xFFFFu), e4m3x2_to_f16x2(w[e] >> 16));
+              for (int n = 0; n < NB; ++n) {
+                mma_f16(s[j][n], f0, f1, f2, f3, qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
+                if constexpr (PAIR) mma_f16(s[j][n], f0, f1, f2, f3, ql[n][i * 4 + e][0], ql[n][i * 4 + e][1]);
+              }
+            }
+          }
         }
-      }
-      // ---- exponents; masked ones are -infinity whatever the bytes were
-      const float xa = fa * ks, xb = fb * ks;
-      const bool whole = __all_sync(ALL_LANES, page >= 0) && t0 + UNIT - 1 <= pos_low && t0 + UNIT <= have &&
-                         (a.window == 0 || t0 > pos_high - a.window || t0 + UNIT <= a.keep);
+        // ---- exponents; masked ones are -infinity whatever the bytes were
+        const float sv = fmaxf(cur.scale.y, 7.888609e-31f);  // 2^-100, the least scale that an append writes
+        const bool odd = cur.scale.y != cur.scale.y;
+        const float ev = odd ? cur.scale.y : __log2f(sv), inv_v = odd ? 1.f : 1.f / sv;
+        const bool whole = __all_sync(ALL_LANES, cur.page >= 0) && t0 + UNIT - 1 <= pos_low && t0 + UNIT <= t.have &&
+                           (a.window == 0 || t0 > pos_high - a.window || t0 + UNIT <= a.keep);
+        uint32_t ph[NB][8], pl[PAIR ? NB : 1][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (PAIR) {
-          s[j][0] += s[j][2];
-          s[j][1] += s[j][3];
-        }
-        s[j][0] = fmaf(s[j][0], xa, ev);
-        s[j][1] = fmaf(s[j][1], xa, ev);
-        s[j][2] = PAIR ? -INFINITY : fmaf(s[j][2], xb, ev);
-        s[j][3] = PAIR ? -INFINITY : fmaf(s[j][3], xb, ev);
-      }
-      if (!whole) {
-        auto seen = [&](int t, int pos) { return page >= 0 && t <= pos && t < have && (a.window == 0 || t > pos - a.window || t < a.keep); };
+        for (int n = 0; n < NB; ++n) {
+          const float f0 = back[n][0] * cur.scale.x, f1 = back[n][1] * cur.scale.x;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 4; ++j) {
+            s[j][n][0] = fmaf(s[j][n][0], f0, ev);
+            s[j][n][1] = fmaf(s[j][n][1], f1, ev);
+            s[j][n][2] = fmaf(s[j][n][2], f0, ev);
+            s[j][n][3] = fmaf(s[j][n][3], f1, ev);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int k = tok + 4 * j + (e & 2), p = pos[n][e & 1];
+                if (!(cur.page >= 0 && k <= p && k < t.have && (a.window == 0 || k > p - a.window || k < a.keep))) s[j][n][e] = -INFINITY;
+              }
+          }
+          // ---- running maximum and denominator
+          float top[2] = {m[n][0], m[n][1]};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            top[0] = fmaxf(top[0], fmaxf(s[j][n][0], s[j][n][2]));
+            top[1] = fmaxf(top[1], fmaxf(s[j][n][1], s[j][n][3]));
+          }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            top[0] = fmaxf(top[0], __shfl_xor_sync(ALL_LANES, top[0], off));
+            top[1] = fmaxf(top[1], __shfl_xor_sync(ALL_LANES, top[1], off));
+          }
+          float down[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int t = tok + 2 * j + e;
-            if (!seen(t, pos_a)) s[j][e] = -INFINITY;
-            if (!PAIR && !seen(t, pos_b)) s[j][2 + e] = -INFINITY;
+            const float base = top[e] == -INFINITY ? 0.f : top[e];
+            down[e] = ex2(m[n][e] - base);
+            m[n][e] = top[e];
+            top[e] = base;
           }
-      }
-      // ---- running maximum and denominator
-      float na = m_a, nb = m_b;
+          float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        na = fmaxf(na, fmaxf(s[j][0], s[j][1]));
-        nb = fmaxf(nb, fmaxf(s[j][2], s[j][3]));
-      }
+          for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int off = 1; off < 4; off <<= 1) {
-        na = fmaxf(na, __shfl_xor_sync(ALL_LANES, na, off));
-        nb = fmaxf(nb, __shfl_xor_sync(ALL_LANES, nb, off));
-      }
-      const float ua = na == -INFINITY ? 0.f : na, ub = nb == -INFINITY ? 0.f : nb;
-      const float ra = ex2(m_a - ua), rb = ex2(m_b - ub);
-      m_a = na;
-      m_b = nb;
-      float sum_a = 0.f, sum_b = 0.f;
+            for (int e = 0; e < 4; ++e) {
+              s[j][n][e] = ex2(s[j][n][e] - top[e & 1]);
+              sum[e & 1] += s[j][n][e];
+            }
+            const uint32_t h0 = pack_f16(s[j][n][0], s[j][n][1]), h1 = pack_f16(s[j][n][2], s[j][n][3]);
+            ph[n][2 * j] = transposed(h0);
+            ph[n][2 * j + 1] = transposed(h1);
+            if constexpr (PAIR) {
+              const float2 r0 = unpack_f16(h0), r1 = unpack_f16(h1);
+              pl[n][2 * j] = transposed(pack_f16(s[j][n][0] - r0.x, s[j][n][1] - r0.y));
+              pl[n][2 * j + 1] = transposed(pack_f16(s[j][n][2] - r1.x, s[j][n][3] - r1.y));
+            }
+          }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        s[j][0] = ex2(s[j][0] - ua);
-        s[j][1] = ex2(s[j][1] - ua);
-        sum_a += s[j][0] + s[j][1];
-        if (!PAIR) {
-          s[j][2] = ex2(s[j][2] - ub);
-          s[j][3] = ex2(s[j][3] - ub);
-          sum_b += s[j][2] + s[j][3];
+          for (int e = 0; e < 2; ++e) l[n][e] = fmaf(sum[e], inv_v, l[n][e] * down[e]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][n][e] *= down[e & 1];
         }
-      }
-      l_a = fmaf(sum_a, inv_v, l_a * ra);
-      if (!PAIR) l_b = fmaf(sum_b, inv_v, l_b * rb);
+        // bytes behind the sequence's end may be anything, and 0 times NaN is NaN
+        const int live = t.have - t0 - cc * 16;
+        const bool cut = !whole && live < 16;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][0] *= ra;
-        o[i][1] *= ra;
-        o[i][2] *= PAIR ? ra : rb;
-        o[i][3] *= PAIR ? ra : rb;
-      }
-      uint32_t p[4][4];
+        for (int i = 0; i < KC; ++i) {
+          const uint32_t from = slot(KC + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float *x = s[2 * e], *y = s[2 * e + 1];
-        p[e][0] = pack_f16(x[0], x[1]);
-        p[e][2] = pack_f16(y[0], y[1]);
-        if (PAIR) {
-          const float2 hx = __half22float2(*reinterpret_cast<__half2*>(&p[e][0])), hy = __half22float2(*reinterpret_cast<__half2*>(&p[e][2]));
-          p[e][1] = pack_f16(x[0] - hx.x, x[1] - hx.y);
-          p[e][3] = pack_f16(y[0] - hy.x, y[1] - hy.y);
-        } else {
-          p[e][1] = pack_f16(x[2], x[3]);
-          p[e][3] = pack_f16(y[2], y[3]);
+          for (int j = 0; j < 4; ++j) {  // head entries of rows r and r + 8
+            uint4 v0 = shared16(from + 2 * j * 512), v1 = shared16(from + (2 * j + 1) * 512);
+            if (cut) {
+              auto keep_bytes = [&](uint32_t& w, int k) { w = live >= k + 4 ? w : live <= k ? 0u : w & ((1u << 8 * (live - k)) - 1); };
+              keep_bytes(v0.x, 0); keep_bytes(v0.y, 4); keep_bytes(v0.z, 8); keep_bytes(v0.w, 12);
+              keep_bytes(v1.x, 0); keep_bytes(v1.y, 4); keep_bytes(v1.z, 8); keep_bytes(v1.w, 12);
+            }
+            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t f0 = e4m3x2_to_f16x2(w0[e] & 0xFFFFu), f1 = e4m3x2_to_f16x2(w1[e] & 0xFFFFu), f2 = e4m3x2_to_f16x2(w0[e] >> 16),
+                             f3 = e4m3x2_to_f16x2(w1[e] >> 16);
+#pragma unroll
+              for (int n = 0; n < NB; ++n) {
+                mma_f16(o[i * 4 + j][n], f0, f1, f2, f3, ph[n][2 * e], ph[n][2 * e + 1]);
+                if constexpr (PAIR) mma_f16(o[i * 4 + j][n], f0, f1, f2, f3, pl[n][2 * e], pl[n][2 * e + 1]);
+              }
+            }
+          }
         }
+        cur = nxt;
       }
-      // bytes behind the sequence's end may be anything, and 0 times NaN is NaN
-      const int live = page >= 0 ? have - tok : 0;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        uint4 v = __ldg(reinterpret_cast<const uint4*>(vp + ((size_t)(8 * i) << c.page_shift)));
-        if (!whole) {
-          auto keep_bytes = [&](uint32_t w, int from) { return live >= from + 4 ? w : live <= from ? 0u : w & ((1u << 8 * (live - from)) - 1); };
-          v.x = keep_bytes(v.x, 0);
-          v.y = keep_bytes(v.y, 4);
-          v.z = keep_bytes(v.z, 8);
-          v.w = keep_bytes(v.w, 12);
-        }
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          mma_f16(o[i], p[e][0], p[e][1], p[e][2], p[e][3], e4m3x2_to_f16x2(w[e] & 0xFFFFu), e4m3x2_to_f16x2(w[e] >> 16));
-      }
-    }
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
-      l_a += __shfl_xor_sync(ALL_LANES, l_a, off);
-      l_b += __shfl_xor_sync(ALL_LANES, l_b, off);
-    }
-    if (PAIR) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][0] += o[i][2];
-        o[i][1] += o[i][3];
-      }
-    }
+          for (int off = 4; off < 32; off <<= 1) l[n][e] += __shfl_xor_sync(ALL_LANES, l[n][e], off);
 
-    // ---- a tile that is complete goes out, a part of one to shared memory
-    if (x0 == 0 && x1 == n) {
-      auto put = [&](int i, float l, float v0, float v1, int d) {
-        if (i >= rows || d >= c.dim) return;
-        const int x = row0 + i, t = x / a.group;
-        T* to = (T*)a.out + (size_t)(r.first + t) * a.out_row + (size_t)(head * a.group + (x - t * a.group)) * c.dim + d;
-        to[0] = from_f32<T>(l == 0.f ? 0.f : v0 / l);
-        to[1] = from_f32<T>(l == 0.f ? 0.f : v1 / l);
-      };
+      // ---- a tile that is complete goes out, a part of one waits for the others
+      if (x0 == 0 && x1 == t.units) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        put(g, l_a, o[i][0], o[i][1], 8 * i + 2 * cc);
-        if (!PAIR) put(g + 8, l_b, o[i][2], o[i][3], 8 * i + 2 * cc);
-      }
-    } else {
-      const int slot = warp * 2 + (x0 == 0 ? 1 : 0);
-      float* w = parts + slot * PART;
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        *reinterpret_cast<float2*>(w + g * DP + 8 * i + 2 * cc) = make_float2(o[i][0], o[i][1]);
-        if (!PAIR) *reinterpret_cast<float2*>(w + (g + 8) * DP + 8 * i + 2 * cc) = make_float2(o[i][2], o[i][3]);
-      }
-      if (cc == 0) {
-        w[ROWS * DP + g] = m_a;
-        w[ROWS * (DP + 1) + g] = l_a;
-        if (!PAIR) {
-          w[ROWS * DP + g + 8] = m_b;
-          w[ROWS * (DP + 1) + g + 8] = l_b;
-        }
-      }
-      // the first unit of the tile names it
-      if (lane == 0) part_tile[slot] = u - x0;
-    }
-    u += x1 - x0;
-    __syncwarp();
-  }
-  __syncthreads();
-
-  // ---- parts of this CTA's warps, tile by tile; they are in the order of the positions
-  for (int first = 0; first < WARPS * 2;) {
-    const int at = part_tile[first];
-    if (at < 0) {
-      ++first;
-      continue;
-    }
-    int end = first + 1;
-    while (end < WARPS * 2 && (part_tile[end] < 0 || part_tile[end] == at)) ++end;
-    int lo = 0, hi = c.seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (unit_end[mid] > at) hi = mid;
-      else lo = mid + 1;
-    }
-    const int b = lo;
-    const SeqRows r = seq_rows(a.row_start, a.rows, b);
-    const Span span = span_of(a, max(a.lens[b], 0), r.n);
-    const int n = span.units(), tiles = tiles_of(r), tile_i = (at - (b ? unit_end[b - 1] : 0)) / n;
-    const int head = tile_i / tiles, tile = tile_i - head * tiles, row0 = tile * ROWS, rows = min(ROWS, r.n * a.group - row0);
-    const bool alone = at >= c0 && at + n <= c1;
-    auto put = [&](int i, int d, float l, float v) {
-      const int x = row0 + i, t = x / a.group;
-      T* to = (T*)a.out + (size_t)(r.first + t) * a.out_row + (size_t)(head * a.group + (x - t * a.group)) * c.dim + d;
-      *to = from_f32<T>(l == 0.f ? 0.f : v / l);
-    };
-    float* mine = a.partials + (size_t)(blockIdx.x * 2 + (at >= c0 ? 1 : 0)) * PART;
-    for (int x = tid; x < rows * DP; x += THREADS) {
-      const int i = x / DP, d = x - i * DP;
-      float m = -INFINITY, l = 0.f, v = 0.f;
-      for (int s = first; s < end; ++s) {
-        if (part_tile[s] < 0) continue;
-        const float* w = parts + s * PART;
-        m = fmaxf(m, w[ROWS * DP + i]);
-      }
-      for (int s = first; s < end; ++s) {
-        if (part_tile[s] < 0) continue;
-        const float* w = parts + s * PART;
-        const float f = m == -INFINITY ? 0.f : ex2(w[ROWS * DP + i] - m);
-        l = fmaf(w[ROWS * (DP + 1) + i], f, l);
-        v = fmaf(w[i * DP + d], f, v);
-      }
-      if (alone) {
-        if (d < c.dim) put(i, d, l, v);
+          for (int e = 0; e < 2; ++e) {
+            const int row = n * 8 + cc * 2 + e, x = t.row0 + row, r = t.n_rows == 1 ? 0 : x / a.group;
+            if (row >= t.rows) continue;
+            T* to = (T*)a.out + (size_t)(t.first_row + r) * a.out_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim;
+            const float f = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              if (16 * i + g < c.dim) to[16 * i + g] = from_f32<T>(o[i][n][e] * f);
+              if (16 * i + g + 8 < c.dim) to[16 * i + g + 8] = from_f32<T>(o[i][n][e + 2] * f);
+            }
+          }
       } else {
-        __stcg(mine + i * DP + d, v);
-        if (d == 0) {
-          __stcg(mine + ROWS * DP + i, m);
-          __stcg(mine + ROWS * (DP + 1) + i, l);
+        __syncwarp();  // all lanes have read their last bytes of the ring
+        float* w = u == u1 ? last_part(warp) : early_part(warp);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = n * 8 + cc * 2 + e;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              w[row * DP + 16 * i + g] = o[i][n][e];
+              w[row * DP + 16 * i + g + 8] = o[i][n][e + 2];
+            }
+            if (g == 0) {
+              w[ROWS * DP + row] = m[n][e];
+              w[ROWS * (DP + 1) + row] = l[n][e];
+            }
+          }
+        if (lane == 0) {
+          part_tile[warp * 2 + (u == u1 ? 1 : 0)] = t.first_unit;
+          part_of_tile[warp * 2 + (u == u1 ? 1 : 0)] = t;
         }
       }
+      copy_wait<0>();  // (nothing but empty groups)
+  }
+  __syncthreads();  // parts in global memory too are read by this block alone
+
+  auto put = [&](const Tile& t, int i, int d, const float4& v, float l) {
+    const int x = t.row0 + i, r = t.n_rows == 1 ? 0 : x / a.group;
+    T* to = (T*)a.out + (size_t)(t.first_row + r) * a.out_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim + d;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    const float w[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < c.dim) to[e] = from_f32<T>(w[e]);
+  };
+  auto add_part = [](float4& v, const float4& p, float f) {
+    v.x = fmaf(p.x, f, v.x);
+    v.y = fmaf(p.y, f, v.y);
+    v.z = fmaf(p.z, f, v.z);
+    v.w = fmaf(p.w, f, v.w);
+  };
+  // ---- parts of this CTA's warps, tile by tile; they are in the order of the positions
+  const int id = lane < WARPS * 2 ? part_tile[lane] : -1;
+  unsigned todo = __ballot_sync(ALL_LANES, id >= 0);
+#pragma unroll 1
+  while (todo) {
+    const int at = __shfl_sync(ALL_LANES, id, __ffs(todo) - 1);
+    const unsigned these = __ballot_sync(ALL_LANES, id == at);
+    todo &= ~these;
+    const Tile& t = part_of_tile[__ffs(these) - 1];
+    const bool alone = at >= c0 && at + t.units <= c1;
+    auto part = [&](int s) -> const float* { return s & 1 ? last_part(s >> 1) : early_part(s >> 1); };
+    // a warp for a row, a lane for a part: the row's maximum, what each part is to be multiplied with, the denominator
+#pragma unroll 1
+    for (int row = warp; row < t.rows; row += WARPS) {
+      const bool in = these >> lane & 1;
+      const float* w = part(in ? lane : __ffs(these) - 1) + ROWS * DP + row;
+      const float m = in ? w[0] : -INFINITY, top = lane_max(m), f = top == -INFINITY || !in ? 0.f : ex2(m - top);
+      const float l = lane_sum(in ? w[ROWS] * f : 0.f);
+      factor[row][lane] = f;
+      if (lane == 0) row_max[row] = top, row_sum[row] = l;
+    }
+    __syncthreads();
+    float* whole = a.partials + (size_t)(blockIdx.x * 2 + (at >= c0 ? 1 : 0)) * PART;
+#pragma unroll 1
+    for (int x = tid; x < t.rows * (DP / 4); x += THREADS) {
+      const int row = x / (DP / 4), d = (x - row * (DP / 4)) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (unsigned rest = these; rest; rest &= rest - 1) {
+        const int s = __ffs(rest) - 1;
+        add_part(v, *reinterpret_cast<const float4*>(part(s) + row * DP + d), factor[row][s]);
+      }
+      if (alone) put(t, row, d, v, row_sum[row]);
+      else __stcg(reinterpret_cast<float4*>(whole + row * DP + d), v);
     }
     if (!alone) {
-      // CTAs that hold a part of the tile: those of its first to its last unit
-      const int first_cta = (int)((((int64_t)at + 1) * ctas - 1) / units), last_cta = (int)((((int64_t)at + n) * ctas - 1) / units);
+      if (tid < t.rows) {
+        __stcg(whole + ROWS * DP + tid, row_max[tid]);
+        __stcg(whole + ROWS * (DP + 1) + tid, row_sum[tid]);
+      }
+      const int first_cta = shares.of(at), n = shares.of(at + t.units - 1) - first_cta + 1;  // CTAs that hold a part of the tile
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        unsigned* counter = a.counters + (size_t)((r.first * (int64_t)a.group / ROWS + b) + tile) * c.kv_heads + head;
-        const bool last = atomicAdd(counter, 1u) == (unsigned)(last_cta - first_cta);
+        unsigned* counter = a.counters + t.counter;
+        const bool last = atomicAdd(counter, 1u) == (unsigned)(n - 1);
         if (last) *counter = 0;  // ready for the next call
         __threadfence();
         last_here = last;
       }
       __syncthreads();
       if (last_here) {
-        auto part_of = [&](int i) { return a.partials + (size_t)(i * 2 + (at >= cta_begin(i) ? 1 : 0)) * PART; };
-        for (int x = tid; x < rows * c.dim; x += THREADS) {
-          const int i = x / c.dim, d = x - i * c.dim;
-          float m = -INFINITY, l = 0.f, v = 0.f;
-          for (int s = first_cta; s <= last_cta; ++s) m = fmaxf(m, __ldcg(part_of(s) + ROWS * DP + i));
-          for (int s = first_cta; s <= last_cta; ++s) {
-            const float* w = part_of(s);
-            const float f = m == -INFINITY ? 0.f : ex2(__ldcg(w + ROWS * DP + i) - m);
-            l = fmaf(__ldcg(w + ROWS * (DP + 1) + i), f, l);
-            v = fmaf(__ldcg(w + i * DP + d), f, v);
+        // of the CTAs' parts only the first can be of a tile that began before its CTA's share
+        const bool split = at < shares.begin(first_cta);
+        auto part_of = [&](int i) { return a.partials + (size_t)((first_cta + i) * 2 + (i == 0 && !split ? 1 : 0)) * PART; };
+#pragma unroll 1
+        for (int row = warp; row < t.rows; row += WARPS) {
+          float top = -INFINITY, l = 0.f;
+#pragma unroll 1
+          for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part_of(i) + ROWS * DP + row));
+          top = lane_max(top);
+#pragma unroll 1
+          for (int i = lane; i < n; i += 32) {
+            const float f = top == -INFINITY ? 0.f : ex2(__ldcg(part_of(i) + ROWS * DP + row) - top);
+            l = fmaf(__ldcg(part_of(i) + ROWS * (DP + 1) + row), f, l);
+            factor[row][i] = f;
           }
-          put(i, d, l, v);
+          l = lane_sum(l);
+          if (lane == 0) row_sum[row] = l;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int x = tid; x < t.rows * (DP / 4); x += THREADS) {
+          const int row = x / (DP / 4), d = (x - row * (DP / 4)) * 4;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int i = 0; i < n; ++i) add_part(v, __ldcg(reinterpret_cast<const float4*>(part_of(i) + row * DP + d)), factor[row][i]);
+          put(t, row, d, v, row_sum[row]);
         }
       }
-      __syncthreads();
     }
-    first = end;
+    __syncthreads();
   }
 }
 
-template <int DP, typename T>
-size_t step_smem(int seqs) {
-  constexpr int WARPS = Shape<DP>::WARPS, ROWS = std::is_same<T, float>::value ? 8 : 16;
-  return (size_t)WARPS * (DP / 16) * 512 + (size_t)WARPS * 2 * ROWS * (DP + 2) * 4 + (size_t)seqs * 4;
+template <int DP, typename T, int NB>
+cudaError_t run(const Kv8AttnArgs& a, int sms, cudaStream_t s) {
+  using S = Shape<DP, NB>;
+  return launch_kernel(kv8_step_kernel<DP, T, NB>, dim3(std::min(sms, KV8_MAX_CTAS)), dim3(S::THREADS), S::SMEM, s, true, a);
 }
-
-template <int DP, typename T>
-cudaError_t run(const Kv8AttnArgs& a, int grid, cudaStream_t s) {
-  return launch_kernel(kv8_step_kernel<DP, T>, dim3(grid), dim3(Shape<DP>::THREADS), step_smem<DP, T>(a.c.seqs), s, false, a);
-}
-template <int DP, typename T>
+template <int DP, typename T, int NB>
 cudaError_t allow() {
-  return cudaFuncSetAttribute(kv8_step_kernel<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)step_smem<DP, T>(KV8_MAX_SEQS));
+  return cudaFuncSetAttribute(kv8_step_kernel<DP, T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP, NB>::SMEM);
 }
-template <typename T>
-cudaError_t run_of(const Kv8AttnArgs& a, int grid, cudaStream_t s) {
+// Tiles of 16 rows read the cache once for what two tiles of 8 would read twice; where registers allow and there are so many.
+template <typename T, int NB>
+cudaError_t run_of(const Kv8AttnArgs& a, int sms, cudaStream_t s) {
   switch (kv8_padded(a.c.dim)) {
-    case 64: return run<64, T>(a, grid, s);
-    case 128: return run<128, T>(a, grid, s);
-    case 192: return run<192, T>(a, grid, s);
-    default: return run<256, T>(a, grid, s);
+    case 64: return run<64, T, NB>(a, sms, s);
+    case 128: return run<128, T, NB>(a, sms, s);
+    case 192: return run<192, T, 1>(a, sms, s);
+    default: return run<256, T, 1>(a, sms, s);
   }
 }
 
 }  // namespace
 
 cudaError_t init_kv8_step_attributes() {
-  cudaError_t all[] = {allow<64, float>(), allow<128, float>(), allow<192, float>(), allow<256, float>(),
-                       allow<64, __nv_bfloat16>(), allow<128, __nv_bfloat16>(), allow<192, __nv_bfloat16>(), allow<256, __nv_bfloat16>()};
+  cudaError_t all[] = {allow<64, float, 1>(), allow<128, float, 1>(), allow<192, float, 1>(), allow<256, float, 1>(), allow<64, __nv_bfloat16, 1>(),
+                       allow<128, __nv_bfloat16, 1>(), allow<192, __nv_bfloat16, 1>(), allow<256, __nv_bfloat16, 1>(),
+                       allow<64, __nv_bfloat16, 2>(), allow<128, __nv_bfloat16, 2>()};
   for (cudaError_t e : all)
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
 
 cudaError_t launch_kv8_attention_step(const Kv8AttnArgs& a, int dtype, int sms, cudaStream_t s) {
-  const int grid = sms < KV8_MAX_CTAS ? sms : KV8_MAX_CTAS;
-  return dtype == PG_DTYPE_F32 ? run_of<float>(a, grid, s) : run_of<__nv_bfloat16>(a, grid, s);
+  if (dtype == PG_DTYPE_F32) return run_of<float, 1>(a, sms, s);
+  return (int64_t)a.group * a.max_rows > 8 ? run_of<__nv_bfloat16, 2>(a, sms, s) : run_of<__nv_bfloat16, 1>(a, sms, s);
 }
 
 }  // namespace pg

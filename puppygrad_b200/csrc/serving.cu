@@ -2,8 +2,9 @@
 // linear_q4.cu and token_logprobs.cu.
 #include "serving.h"
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
-#include <mutex>
 #include <string>
 
 #include "common.h"
@@ -17,9 +18,18 @@ namespace {
 class DeviceScope {
  public:
   explicit DeviceScope(int device) {
+    if (device < 0 || device >= MAX_DEVICES) {
+      rc_ = set_error(PG_INVALID_INPUT, "device " + std::to_string(device) + " out of range");
+      return;
+    }
     if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
+    sms_ = sms_of_[device].load(std::memory_order_acquire);
+    if (sms_ && before_ == device) {  // nothing to change, nothing to put back
+      before_ = -1;
+      return;
+    }
     rc_ = ensure_device(device);
-    if (rc_ == PG_OK) rc_ = init(device);
+    if (rc_ == PG_OK && !sms_) rc_ = init(device);
   }
   ~DeviceScope() {
     if (before_ >= 0) cudaSetDevice(before_);
@@ -28,25 +38,21 @@ class DeviceScope {
   int sms() const { return sms_; }
 
  private:
+  static constexpr int MAX_DEVICES = 64;
+  static std::atomic<int> sms_of_[MAX_DEVICES];  // 0: no call on that device yet
   int init(int device) {
-    static std::mutex mu;
-    static int sms[64];
-    std::lock_guard<std::mutex> g(mu);
-    if (device >= 64) return set_error(PG_INVALID_INPUT, "device " + std::to_string(device) + " out of range (64 at most)");
-    if (!sms[device]) {
-      int n = 0;
-      cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
-      if (e == cudaSuccess) e = init_kv8_append_attributes();
-      if (e == cudaSuccess) e = init_kv8_step_attributes();
-      if (e == cudaSuccess) e = init_q4_attributes();
-      if (e != cudaSuccess) return set_error(PG_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
-      sms[device] = n;
-    }
-    sms_ = sms[device];
+    cudaError_t e = cudaDeviceGetAttribute(&sms_, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = init_kv8_append_attributes();
+    if (e == cudaSuccess) e = init_kv8_step_attributes();
+    if (e == cudaSuccess) e = init_kv8_portion_attributes();
+    if (e == cudaSuccess) e = init_q4_attributes();
+    if (e != cudaSuccess) return set_error(PG_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
+    sms_of_[device].store(sms_, std::memory_order_release);
     return PG_OK;
   }
   int before_ = -1, rc_ = PG_OK, sms_ = 0;
 };
+std::atomic<int> DeviceScope::sms_of_[MAX_DEVICES];
 
 int launched(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return PG_OK;
@@ -102,13 +108,15 @@ Kv8View view(const pg_kv8_cache* c) {
           c->kv_heads, c->head_dim, c->seqs, c->pages_per_seq};
 }
 
-// Counters of the step kernel, one for each tile of rows that several CTAs may share, then two partial tiles for every CTA.
-size_t counter_bytes(const pg_kv8_cache* c, int rows, int heads, int dtype) {
-  const int64_t tiles = ((int64_t)rows * (heads / c->kv_heads) / kv8_tile_rows(dtype) + c->seqs) * c->kv_heads;
+// Counters of the step kernel, one for each tile of (at least 8) rows that several CTAs may share, then parts of tiles: two for every
+// CTA and one for each of its warps, of which there are 16 with tiles of 8 rows, 8 with tiles of 16.
+size_t counter_bytes(const pg_kv8_cache* c, int rows, int heads) {
+  const int64_t tiles = ((int64_t)rows * (heads / c->kv_heads) / 8 + c->seqs) * c->kv_heads;
   return ((size_t)tiles * 4 + 255) / 256 * 256;
 }
-size_t partial_bytes(const pg_kv8_cache* c, int dtype) {
-  return (size_t)KV8_MAX_CTAS * 2 * kv8_tile_rows(dtype) * (kv8_padded(c->head_dim) + 2) * 4;
+size_t partial_bytes(const pg_kv8_cache* c) {
+  const int padded = kv8_padded(c->head_dim), rows = padded == 64 ? (2 + 16) * 16 : std::max((2 + 16) * 8, (2 + 8) * 16);
+  return (size_t)KV8_MAX_CTAS * rows * (padded + 2) * 4;
 }
 
 }  // namespace
@@ -154,7 +162,7 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
 uint64_t pg_kv8_attention_workspace_bytes(const pg_kv8_cache* cache, int32_t rows, int32_t heads, int32_t dtype) {
   if (check_cache(cache) || check_dtype(dtype) || check_heads(cache, heads)) return 0;
   if (rows < 0) return bad("rows must not be negative"), 0;
-  return counter_bytes(cache, rows, heads, dtype) + partial_bytes(cache, dtype);
+  return counter_bytes(cache, rows, heads) + partial_bytes(cache);
 }
 
 int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, void* out, int64_t out_row, int32_t dtype,
@@ -177,14 +185,19 @@ int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, vo
   if (!aligned(workspace, 256)) return bad("workspace is not 256-byte aligned");
   // pieces of 64 tokens of all tiles of rows are numbered with 31 bits
   const int group = heads / cache->kv_heads;
-  const int64_t tiles = ((int64_t)rows * group / kv8_tile_rows(dtype) + cache->seqs) * cache->kv_heads;
+  const int64_t tiles = ((int64_t)rows * group / 8 + cache->seqs) * cache->kv_heads;
   if (tiles * (((int64_t)cache->pages_per_seq * cache->page_tokens + 63) / 64) > INT32_MAX)
     return bad("rows " + std::to_string(rows) + " with tables of " + std::to_string(cache->pages_per_seq) + " pages are too many for one call");
   DeviceScope scope(cache->device);
   if (scope.rc()) return scope.rc();
+  // rows that fill less than half a tile of the portion kernel, and all of them where it has no table of rows
+  const bool portions = row_start && (int64_t)group * max_rows > KV8_STEP_ROWS;
   Kv8AttnArgs a{view(cache), q, out, q_row, out_row, heads, group, rows, max_rows, row_start, lens, scale, window, window > 0 ? keep_first : 0,
-                (unsigned*)workspace, (float*)((char*)workspace + counter_bytes(cache, rows, heads, dtype))};
-  return launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention");
+                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)workspace, (float*)((char*)workspace + counter_bytes(cache, rows, heads))};
+  if (!portions) return launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention");
+  a.max_rows = std::min(max_rows, (KV8_STEP_ROWS + group - 1) / group);
+  if (int r = launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention")) return r;
+  return launched(launch_kv8_attention_portion(a, dtype, (cudaStream_t)stream), "kv8_attention");
 }
 
 uint64_t pg_q4_packed_bytes(int32_t n, int32_t k) {

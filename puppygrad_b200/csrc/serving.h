@@ -9,7 +9,8 @@
 namespace pg {
 
 constexpr int KV8_MAX_SEQS = 4096;
-constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace must not hang on the device
+constexpr int KV8_STEP_ROWS = 64;
+constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace does not hang on the device
 
 __host__ __device__ inline int kv8_padded(int head_dim) { return (head_dim + 63) / 64 * 64; }
 
@@ -39,6 +40,7 @@ struct Kv8AttnArgs {
   const int *row_start, *lens;
   float scale;
   int window, keep;
+  int step_rows;  // sequences of at most so many (token, head of the group) rows are the step kernel's, the others the portion kernel's
   unsigned* counters;
   float* partials;
 };
@@ -60,14 +62,13 @@ struct LogprobArgs {
   float* top_logprobs;
 };
 
-// Rows of a tile of the step kernel: FP32 queries take two MMA rows each.
-inline int kv8_tile_rows(int dtype) { return dtype == PG_DTYPE_F32 ? 8 : 16; }
-
 cudaError_t init_kv8_append_attributes();
 cudaError_t init_kv8_step_attributes();
+cudaError_t init_kv8_portion_attributes();
 cudaError_t init_q4_attributes();
 cudaError_t launch_kv8_append(const Kv8AppendArgs& a, int dtype, cudaStream_t s);
 cudaError_t launch_kv8_attention_step(const Kv8AttnArgs& a, int dtype, int sms, cudaStream_t s);
+cudaError_t launch_kv8_attention_portion(const Kv8AttnArgs& a, int dtype, cudaStream_t s);
 cudaError_t launch_quantize_q4(const void* w, int64_t w_row, int dtype, int n, int k, int group, uint8_t* packed, uint16_t* scales, cudaStream_t s);
 cudaError_t launch_linear_q4(const Q4Args& a, int dtype, int sms, cudaStream_t s);
 cudaError_t launch_token_logprobs(const LogprobArgs& a, int dtype, int sms, cudaStream_t s);

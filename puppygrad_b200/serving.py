@@ -1,19 +1,27 @@
 """Operators of a serving program on its own device buffers: a paged cache of keys and values in 8 bits, products with 4-bit weights, log
 probabilities of given tokens. include/puppygrad_b200.h has the layouts and what each call promises.
 
-Buffers are anything with the interface of a torch tensor (`data_ptr`, `shape`, `stride`, `dtype`, `device`); torch itself is not
-imported. Calls are enqueued on `stream` (a CUDA stream's address, 0 = the default stream) and return without waiting; what they
+Buffers are anything with the interface of a torch tensor (`data_ptr`, `shape`, `stride`, `is_contiguous`, `dtype`, `get_device`); torch
+itself is not imported. Calls are enqueued on `stream` (a CUDA stream's address, 0 = the default stream) and return without waiting; what they
 read must stay allocated until they have run.
 """
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+from typing import Any, Dict, Optional, Tuple
 
 from . import _native as N
 from .errors import Gpt2Error, check
 
-_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1}
+_CODES = {"torch.float32": 0, "torch.bfloat16": 1}
+_seen: Dict[Any, Optional[str]] = {}  # names of dtype objects: printing one takes longer than all of a tensor's other checks
+
+
+def _name(dtype) -> str:
+    name = _seen.get(dtype)
+    if name is None:
+        name = _seen[dtype] = str(dtype)
+    return name
 
 
 def _bad(what: str):
@@ -21,41 +29,43 @@ def _bad(what: str):
 
 
 def _code(t, name: str) -> int:
-    code = _DTYPES.get(str(t.dtype))
+    code = _CODES.get(_name(t.dtype))
     if code is None:
         raise _bad(f"{name}: dtype {t.dtype} must be float32 or bfloat16")
     return code
 
 
 def _device(t, name: str) -> int:
-    if t.device.type != "cuda":
+    device = t.get_device()
+    if device < 0:
         raise _bad(f"{name} is on {t.device}, a CUDA device is needed")
-    return t.device.index
+    return device
 
 
 def _flat(t, name: str, dtype: str, shape: Tuple[int, ...], device: int) -> int:
     """Address of a buffer that has to be contiguous and of that type and shape."""
-    if str(t.dtype) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or _name(t.dtype) != dtype or not t.is_contiguous():
         raise _bad(f"{name}: {dtype} {shape} without gaps is needed, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
-    if _device(t, name) != device:
+    if t.get_device() != device:
         raise _bad(f"{name} is on {t.device}, the others are on cuda:{device}")
     return t.data_ptr()
 
 
-def _rows(t, name: str, dtype, inner: Tuple[int, ...], device: int, rows: Optional[int] = None) -> Tuple[int, int]:
+def _rows(t, name: str, dtype, inner: Tuple[int, ...], device: int, rows: int) -> Tuple[int, int]:
     """Address and distance between rows of [rows, *inner], whose rows are without gaps."""
-    shape, stride = tuple(t.shape), t.stride()
-    if shape[1:] != inner or (rows is not None and shape[0] != rows) or t.dtype != dtype:
-        raise _bad(f"{name}: {dtype} [{'rows' if rows is None else rows}, {', '.join(map(str, inner))}] is needed, got {t.dtype} {shape}")
-    width = 1
-    for n, s in zip(reversed(inner), reversed(stride[1:])):
-        if n > 1 and s != width:
-            raise _bad(f"{name}: a row must be without gaps, got strides {stride}")
-        width *= n
-    if _device(t, name) != device:
+    if t.shape != (rows, *inner) or t.dtype != dtype:
+        raise _bad(f"{name}: {dtype} {(rows, *inner)} is needed, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != device:
         raise _bad(f"{name} is on {t.device}, the others are on cuda:{device}")
+    stride, width = t.stride(), inner[-1]
+    gap = width > 1 and stride[-1] != 1
+    if len(inner) == 2:
+        gap = gap or (inner[0] > 1 and stride[1] != width)
+        width *= inner[0]
+    if gap:
+        raise _bad(f"{name}: a row must be without gaps, got strides {stride}")
     # of a single row (or none) the distance says nothing
-    return t.data_ptr(), stride[0] if shape[0] > 1 else width
+    return t.data_ptr(), stride[0] if rows > 1 else width
 
 
 class Kv8Cache:
@@ -95,7 +105,7 @@ class Kv8Cache:
         length with them."""
         rows, inner, device = k.shape[0], (self.kv_heads, self.head_dim), self.device
         dtype = _code(k, "k")
-        kp, ks = _rows(k, "k", k.dtype, inner, device)
+        kp, ks = _rows(k, "k", k.dtype, inner, device, rows)
         vp, vs = _rows(v, "v", k.dtype, inner, device, rows)
         qp = qs = op = os = heads = 0
         if q is not None or q_out is not None:
@@ -109,7 +119,7 @@ class Kv8Cache:
 
     def workspace_bytes(self, rows: int, heads: int, dtype) -> int:
         """Size of the workspace of `attention` calls of up to that many rows; its memory must be zero before its first use."""
-        code = _DTYPES.get(str(dtype), -1)
+        code = _CODES.get(_name(dtype), -1)
         size = N.lib.pg_kv8_attention_workspace_bytes(self._ref, rows, heads, code)
         if not size:
             raise _bad(N.lib.pg_last_error_message().decode())
@@ -122,7 +132,7 @@ class Kv8Cache:
         before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each."""
         rows, heads = q.shape[0], q.shape[1]
         dtype, inner = _code(q, "q"), (heads, self.head_dim)
-        qp, qs = _rows(q, "q", q.dtype, inner, self.device)
+        qp, qs = _rows(q, "q", q.dtype, inner, self.device, rows)
         op, os = _rows(out, "out", q.dtype, inner, self.device, rows)
         lp, sp = self._row_map(lens, row_start)
         wp = _flat(workspace, "workspace", "torch.uint8", (workspace.shape[0],), self.device)
@@ -132,8 +142,7 @@ class Kv8Cache:
 
 def q4_shapes(n: int, k: int, group: int) -> Tuple[Tuple[int, int, int], Tuple[int, int]]:
     """Shapes of the packed codes (uint8) and the scales (bfloat16) of a 4-bit matrix of n outputs and k inputs."""
-    size = N.lib.pg_q4_scale_bytes(n, k, group)
-    if not size:
+    if not N.lib.pg_q4_scale_bytes(n, k, group):
         raise _bad(N.lib.pg_last_error_message().decode())
     return (-(-n // 16), -(-k // 64), 512), (-(-k // group), -(-n // 16) * 16)
 
@@ -142,7 +151,7 @@ def quantize_q4(w, packed, scales, group: int, stream: int = 0) -> None:
     """Lays the matrix w [n, k] out in 4 bits, with one scale for every `group` (64 or 128) inputs of an output."""
     n, k = w.shape
     dtype, device = _code(w, "w"), _device(w, "w")
-    wp, ws = _rows(w, "w", w.dtype, (k,), device)
+    wp, ws = _rows(w, "w", w.dtype, (k,), device, n)
     ps, ss = q4_shapes(n, k, group)
     check(N.lib.pg_quantize_q4(wp, ws, dtype, n, k, group, _flat(packed, "packed", "torch.uint8", ps, device),
                                _flat(scales, "scales", "torch.bfloat16", ss, device), device, stream))
@@ -153,10 +162,10 @@ def linear_q4(x, packed, scales, out, group: int, bias=None, stream: int = 0) ->
     m, k = x.shape
     n = out.shape[1]
     dtype, device = _code(x, "x"), _device(x, "x")
-    xp, xs = _rows(x, "x", x.dtype, (k,), device)
+    xp, xs = _rows(x, "x", x.dtype, (k,), device, m)
     op, os = _rows(out, "out", x.dtype, (n,), device, m)
-    ps, ss = q4_shapes(n, k, group)
-    bp = 0 if bias is None else _flat(bias, "bias", str(x.dtype), (n,), device)
+    ps, ss = (-(-n // 16), -(-k // 64), 512), (-(-k // group) if group > 0 else 0, -(-n // 16) * 16)
+    bp = 0 if bias is None else _flat(bias, "bias", _name(x.dtype), (n,), device)
     check(N.lib.pg_linear_q4(xp, xs, _flat(packed, "packed", "torch.uint8", ps, device), _flat(scales, "scales", "torch.bfloat16", ss, device), bp,
                              dtype, m, n, k, group, op, os, device, stream))
 
@@ -166,12 +175,12 @@ def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=No
     log probabilities [rows, k] (k up to 32), each where its output is given."""
     rows, vocab = logits.shape
     dtype, device = _code(logits, "logits"), _device(logits, "logits")
-    lp, ls = _rows(logits, "logits", logits.dtype, (vocab,), device)
+    lp, ls = _rows(logits, "logits", logits.dtype, (vocab,), device, rows)
     if (top_ids is None) != (top_logprobs is None):
         raise _bad("top_ids and top_logprobs must be given together")
     k = 0 if top_ids is None else top_ids.shape[1]
     f = lambda t, name, kind, shape: 0 if t is None else _flat(t, name, kind, shape, device)
-    check(N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, f(targets, "targets", "torch.int32", (rows,)),
-                                  f(logprobs, "logprobs", "torch.float32", (rows,)), f(entropy, "entropy", "torch.float32", (rows,)), k,
-                                  f(top_ids, "top_ids", "torch.int32", (rows, k)), f(top_logprobs, "top_logprobs", "torch.float32", (rows, k)),
-                                  device, stream))
+    each = (rows,)
+    check(N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, f(targets, "targets", "torch.int32", each), f(logprobs, "logprobs", "torch.float32", each),
+                                  f(entropy, "entropy", "torch.float32", each), k, f(top_ids, "top_ids", "torch.int32", (rows, k)),
+                                  f(top_logprobs, "top_logprobs", "torch.float32", (rows, k)), device, stream))

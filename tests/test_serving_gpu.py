@@ -102,6 +102,15 @@ ATTENTION = [
     ([1000, 300, 64, 10], [3, 200, 64, 2], 8, 4, 64, 16, 100, 70),
     ([1000, 131], [1, 60], 4, 1, 128, 32, 1, 0),  # each row sees itself alone
     ([900], [1], 4, 4, 64, 64, 1000, 5),
+    # many rows of a sequence
+    ([500, 260, 3], [300, 260, 1], 6, 2, 96, 32, 0, 0),
+    ([300], [129], 2, 2, 256, 64, 0, 0),
+    ([200], [200], 5, 1, 192, 16, 0, 0),
+    ([70, 1000], [70, 65], 16, 1, 64, 64, 0, 0),
+    ([50, 0, 64], [200, 100, 128], 2, 2, 128, 16, 0, 0),  # more rows than tokens, and rows of an empty sequence
+    ([1500, 90], [700, 1], 4, 2, 80, 64, 333, 70),
+    ([600], [600], 3, 1, 2, 32, 5, 0),
+    ([777, 512], [500, 512], 8, 8, 64, 64, 0, 0),
 ]
 
 
