@@ -239,12 +239,15 @@ APPEND = [
     ([40, 100], [15, 33], 5, 1, 80, 32, 2),
     ([300], [290], 2, 2, 256, 64, 256),
     ([70], [70], 3, 3, 2, 16, 2),
+    ([100, 3], [60, 3], 4, 2, 192, 32, 96),
+    ([65, 64], [2, 64], 4, 1, 64, 16, 32),
 ]
 
 
+@pytest.mark.parametrize("odd", [True, False])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("lens,rows,heads,kvh,dim,page,rot", APPEND)
-def test_append(lens, rows, heads, kvh, dim, page, rot, dtype):
+def test_append(lens, rows, heads, kvh, dim, page, rot, dtype, odd):
     before = [n - r for n, r in zip(lens, rows)]
     cache = Cache(before, kvh, dim, page, 40 + sum(lens), spare=3 + sum(-(-n // page) for n in lens))
     free = [p for p in range(cache.pool.shape[0]) if p not in set(cache.table.flatten().tolist())]
@@ -258,8 +261,9 @@ def test_append(lens, rows, heads, kvh, dim, page, rot, dtype):
     handle = pg.Kv8Cache(cache.pool, cache.scales, table, page_tokens=page, head_dim=dim)
     total = sum(rows)
     # rows of a product with more outputs than these: gaps between rows, odd addresses
-    wide = (torch.randn(total, (heads + 2 * kvh) * dim + 5, generator=gen(1), device=DEV) * 1.7).to(dtype)
-    qkv = wide[:, 1:1 + (heads + 2 * kvh) * dim].view(total, heads + 2 * kvh, dim)
+    gap = 5 if odd else 8
+    wide = (torch.randn(total, (heads + 2 * kvh) * dim + gap, generator=gen(1), device=DEV) * 1.7).to(dtype)
+    qkv = wide[:, gap // 5 * odd:][:, :(heads + 2 * kvh) * dim].view(total, heads + 2 * kvh, dim)
     q, k, v = qkv[:, :heads], qkv[:, heads:heads + kvh], qkv[:, heads + kvh:]
     old_pool, old_scales, before_q = cache.pool.clone(), cache.scales.clone(), q.double()
     old = [ref.sequence_kv(old_pool, old_scales, table[b], n, page, dim) for b, n in enumerate(before)]
