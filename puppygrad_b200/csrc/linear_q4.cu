@@ -2,16 +2,22 @@
 //
 // out[m][n] = sum over groups of scale[group][n] * sum_k (code[n][k] - 8) x[m][k]. Bound: memory, half a byte for every weight; at that
 // rate an SM gets 46 weights a clock, too many for multiply-adds of every row (128 lanes a clock), so the products are m16n8k16 matrix
-// instructions with 16 outputs as rows and 8 tokens as columns, on codes turned into 16-bit floats in registers: a field of 4 bits or-ed
-// into the mantissa of 2^7 (BF16) or 2^10 (FP16) is that power plus the code, one subtraction gives the exact weight. Order of k
-// within a tile is free as long as both operands agree: a lane takes 16 consecutive inputs (k steps of 4), so it loads 16 bytes of
-// weights (8 of outputs r and of r + 8) and 16 inputs in a row.
-// BF16 inputs are exact operands. FP32 inputs are pairs of FP16 numbers, scaled by a power of two for every 64 inputs of a row, whose
-// two halves are separate columns: FP32 grade. A group's sums are FP32, times the scale once per 64 inputs.
-// A CTA has R tiles of 16 outputs; its warps take every eighth tile of 64 inputs and are added up in shared memory, in order.
+// instructions with 16 outputs as rows and 8 tokens as columns, on codes turned into 16-bit floats in registers. Order of k within a
+// tile is free as long as both operands agree: a lane takes 16 consecutive inputs (k steps of 4), so it loads 16 bytes of weights
+// (8 of outputs r and of r + 8) and 16 inputs in a row.
+//  - BF16 inputs are exact operands; a field of 4 bits or-ed into the mantissa of 128 is 128 + code.
+//  - FP32 inputs are pairs of FP16 numbers, scaled by a power of two for every 64 inputs of a row, two products into one accumulator:
+//    FP32 grade. A field of 4 bits at the low end of an FP16 mantissa is the subnormal code * 2^-24, one place further up 16
+//    times that, which inputs scaled by 16 and by 1 make up for: one instruction for two weights.
+// Neither subtracts 8 (or 136) from every weight: the accumulators start at -8 (-136) * sum x, which one more product with a constant
+// operand gives in the accumulators' own layout, once for all the outputs of a CTA. A group's sums are FP32, times the scale
+// once per 64 inputs.
+// A CTA has a range of the tiles of 16 outputs and goes over it in passes of up to R tiles, so that 64 inputs once loaded serve R tiles. Its
+// warps take every WARPS-th tile of 64 inputs and are added up in shared memory, in order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "device_util.cuh"
@@ -20,172 +26,204 @@
 namespace pg {
 namespace {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-
 template <bool PAIR>
-__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   if (PAIR)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Inputs 2 i and 2 i + 1 of a word of 8 codes, as exact 16-bit floats.
+// Inputs 2 i and 2 i + 1 of a word of 8 codes as 16-bit floats. FP16: code * 2^-24 for even i, code * 2^-20 for odd i.
 template <bool PAIR>
 __device__ __forceinline__ uint32_t weights2(uint32_t word, int i) {
-  if (PAIR) {
-    const uint32_t u = ((word >> (4 * i)) & 0x000F000Fu) | 0x64006400u;  // 1024 + code
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1032.f));
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const uint32_t u = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
-  const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(136.f));
-  return *reinterpret_cast<const uint32_t*>(&h);
+  if (PAIR) return (i < 2 ? word : word >> 8) & (i & 1 ? 0x00F000F0u : 0x000F000Fu);
+  return ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
 }
 
-// 16 inputs of one row as operand words: word 2 s + e holds inputs 4 s + 2 e and 4 s + 2 e + 1.
+// 16 inputs of one row: as they come, and as operand words (word 2 s + e: inputs 4 s + 2 e and 4 s + 2 e + 1).
 template <typename T>
-struct Inputs;
-template <>
-struct Inputs<__nv_bfloat16> {
-  uint32_t w[8];
-  __device__ __forceinline__ void load(const __nv_bfloat16* p, int live, bool wide) {
+struct Raw {
+  uint4 v[sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, int live, bool wide) {
+    constexpr int N = 16 / sizeof(T);
     if (wide && live >= 16) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 8);
-      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-      w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-    } else {
-      const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = (2 * i < live ? (uint32_t)u[2 * i] : 0u) | (2 * i + 1 < live ? (uint32_t)u[2 * i + 1] << 16 : 0u);
+      for (int i = 0; i < (int)sizeof(T); ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * N);
+    } else {
+      union {
+        uint4 u[sizeof(T)];
+        T t[16];
+      } x;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.t[i] = i < live ? p[i] : from_f32<T>(0.f);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); ++i) v[i] = x.u[i];
     }
   }
 };
+template <typename T>
+struct Operand;
 template <>
-struct Inputs<float> {
-  uint32_t hi[8], lo[8];
-  float back;  // what the row's sums of these 64 inputs are to be multiplied with
-  __device__ __forceinline__ void load(const float* p, int live, bool wide) {
-    float v[16];
-    if (wide && live >= 16) {
+struct Operand<__nv_bfloat16> {
+  uint32_t w[1][8];
+  __device__ __forceinline__ float make(const Raw<__nv_bfloat16>& r) {
+    w[0][0] = r.v[0].x; w[0][1] = r.v[0].y; w[0][2] = r.v[0].z; w[0][3] = r.v[0].w;
+    w[0][4] = r.v[1].x; w[0][5] = r.v[1].y; w[0][6] = r.v[1].z; w[0][7] = r.v[1].w;
+    return 1.f;
+  }
+};
+template <>
+struct Operand<float> {
+  uint32_t w[2][8];
+  // What the row's sums of these 64 inputs are to be multiplied with.
+  __device__ __forceinline__ float make(const Raw<float>& r) {
+    float v[16], m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 f = *reinterpret_cast<const float4*>(p + 4 * i);
-        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = i < live ? p[i] : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      v[4 * i] = __uint_as_float(r.v[i].x); v[4 * i + 1] = __uint_as_float(r.v[i].y);
+      v[4 * i + 2] = __uint_as_float(r.v[i].z); v[4 * i + 3] = __uint_as_float(r.v[i].w);
     }
-    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
     m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 1));
     m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 2));
     const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
-    const float s = __uint_as_float((uint32_t)(127 - e) << 23);
-    back = __uint_as_float((uint32_t)(127 + e) << 23);
+    const float s = __uint_as_float((uint32_t)(127 - e) << 23), s16 = 16.f * s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float a = v[2 * i] * s, b = v[2 * i + 1] * s;
+      const float f = i & 1 ? s : s16, a = v[2 * i] * f, b = v[2 * i + 1] * f;
       const __half2 h = __floats2half2_rn(a, b);
-      const float2 f = __half22float2(h);
-      const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-      lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+      const float2 q = __half22float2(h);
+      const __half2 l = __floats2half2_rn(a - q.x, b - q.y);
+      w[0][i] = *reinterpret_cast<const uint32_t*>(&h);
+      w[1][i] = *reinterpret_cast<const uint32_t*>(&l);
     }
+    return __uint_as_float((uint32_t)(127 + e + 20) << 23);
   }
 };
 
-// NT: groups of 8 tokens.
-template <typename T, int NT, int R>
-__global__ void __launch_bounds__(THREADS) linear_q4_kernel(Q4Args a) {
+// NT: groups of 8 tokens. R: tiles of 16 outputs of a pass.
+template <typename T, int NT, int WARPS, int R>
+__global__ void __launch_bounds__(WARPS * 32, 1) linear_q4_kernel(Q4Args a) {
   constexpr bool PAIR = std::is_same<T, float>::value;
-  __shared__ float sums[WARPS][R * 16][NT * 8 + 1];
+  constexpr int THREADS = WARPS * 32, PARTS = PAIR ? 2 : 1, LD = NT * 8 + 1;
+  extern __shared__ float sums[];  // [WARPS][R * 16][LD]
+  grid_dep_launch();
+  grid_dep_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const int row_tiles = (a.n + 15) >> 4, k_tiles = (a.k + 63) >> 6, t0 = blockIdx.x * R, ld = row_tiles * 16, shift = a.group == 128 ? 1 : 0;
+  const int row_tiles = (a.n + 15) >> 4, k_tiles = (a.k + 63) >> 6, ld = row_tiles * 16, shift = a.group == 128 ? 1 : 0;
+  // this CTA's tiles, cut into passes of nearly equal size
+  const int each = row_tiles / gridDim.x, more = row_tiles - each * gridDim.x;
+  const int t_first = blockIdx.x * each + min((int)blockIdx.x, more), t_count = each + ((int)blockIdx.x < more ? 1 : 0);
+  const int passes = (t_count + R - 1) / R, per_pass = (t_count + passes - 1) / passes;
   const bool wide = ((uintptr_t)a.x & 15) == 0 && (a.x_row * sizeof(T)) % 16 == 0;
-  float acc[R][NT][4];
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[r][t][e] = 0.f;
 
-  for (int kt = warp; kt < k_tiles; kt += WARPS) {
+  struct Loads {
     uint4 w[R];
-    float sa[R], sb[R];
+    uint16_t s[R][2];
+    Raw<T> x[NT];
+  };
+  auto load = [&](Loads& l, int t0, int kt) {
+    const uint4* w = reinterpret_cast<const uint4*>(a.packed + ((size_t)t0 * k_tiles + kt) * 512) + lane;
+    const uint16_t* s = a.scales + (size_t)(kt >> shift) * ld + t0 * 16 + g;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int t = min(t0 + r, row_tiles - 1);
-      w[r] = __ldg(reinterpret_cast<const uint4*>(a.packed + ((size_t)t * k_tiles + kt) * 512) + lane);
-      const uint16_t* s = a.scales + (size_t)(kt >> shift) * ld + t * 16 + g;
-      sa[r] = __uint_as_float((uint32_t)__ldg(s) << 16);
-      sb[r] = __uint_as_float((uint32_t)__ldg(s + 8) << 16);
-    }
-    Inputs<T> x[NT];
+    for (int r = 0; r < R; ++r)
+      if (r == 0 || (r < per_pass && t0 + r < t_first + t_count)) {
+        l.w[r] = __ldg(w + (size_t)r * k_tiles * 32);
+        l.s[r][0] = __ldg(s + r * 16);
+        l.s[r][1] = __ldg(s + r * 16 + 8);
+      }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int tok = t * 8 + g, from = kt * 64 + c * 16;
-      x[t].load((const T*)a.x + (size_t)min(tok, a.m - 1) * a.x_row + from, tok < a.m ? a.k - from : 0, wide);
+      l.x[t].load((const T*)a.x + min(tok, a.m - 1) * a.x_row + from, tok < a.m ? a.k - from : 0, wide);
     }
+  };
+  Loads now, next;
+  if (warp < k_tiles) load(now, t_first, warp);
+#pragma unroll 1
+  for (int t0 = t_first; t0 < t_first + t_count; t0 += per_pass) {
+    const int tiles = min(per_pass, t_first + t_count - t0);
+    float acc[R][NT][4];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float hi[NT][4], lo[NT][4];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) hi[t][e] = lo[t][e] = 0.f;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        // inputs 4 s .. 4 s + 3 of outputs g (words x, y) and g + 8 (z, w)
-        const uint32_t wa = s < 2 ? w[r].x : w[r].y, wb = s < 2 ? w[r].z : w[r].w;
-        const uint32_t f[4] = {weights2<PAIR>(wa, (s & 1) * 2), weights2<PAIR>(wb, (s & 1) * 2), weights2<PAIR>(wa, (s & 1) * 2 + 1),
-                               weights2<PAIR>(wb, (s & 1) * 2 + 1)};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if constexpr (PAIR) {
-            mma16<true>(hi[t], f, x[t].hi[2 * s], x[t].hi[2 * s + 1]);
-            mma16<true>(lo[t], f, x[t].lo[2 * s], x[t].lo[2 * s + 1]);
-          } else {
-            mma16<false>(hi[t], f, x[t].w[2 * s], x[t].w[2 * s + 1]);
-          }
-        }
-      }
+        for (int e = 0; e < 4; ++e) acc[r][t][e] = 0.f;
+#pragma unroll 1
+    for (int kt = warp; kt < k_tiles; kt += WARPS) {
+      // the next tile of inputs, or the next pass's first one
+      if (kt + WARPS < k_tiles) load(next, t0, kt + WARPS);
+      else if (t0 + per_pass < t_first + t_count) load(next, t0 + per_pass, warp);
+      Operand<T> x[NT];
+      float base[NT][4], back[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float b0 = 1.f, b1 = 1.f;
-        if constexpr (PAIR) {  // columns 2 c and 2 c + 1 are the tokens of lanes 8 c and 8 c + 4
-          b0 = __shfl_sync(ALL_LANES, x[t].back, c * 8);
-          b1 = __shfl_sync(ALL_LANES, x[t].back, c * 8 + 4);
+        const float b = x[t].make(now.x[t]);
+        if (PAIR) {  // columns 2 c and 2 c + 1 are the tokens of lanes 8 c and 8 c + 4
+          back[t][0] = __shfl_sync(ALL_LANES, b, c * 8);
+          back[t][1] = __shfl_sync(ALL_LANES, b, c * 8 + 4);
         }
+        const uint32_t even = PAIR ? 0x80088008u : 0xC308C308u, odd = PAIR ? 0x80808080u : 0xC308C308u;  // -8 in either place; -136
+        const uint32_t f[4] = {even, even, odd, odd};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = PAIR ? (hi[t][e] + lo[t][e]) * (e & 1 ? b1 : b0) : hi[t][e];
-          acc[r][t][e] = fmaf(v, e < 2 ? sa[r] : sb[r], acc[r][t][e]);
-        }
+        for (int e = 0; e < 4; ++e) base[t][e] = 0.f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+          for (int s = 0; s < 4; ++s) mma16<PAIR>(base[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
       }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r > 0 && r >= tiles) continue;
+        float d[NT][4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          // inputs 4 s .. 4 s + 3 of outputs g (words x, y) and g + 8 (z, w)
+          const uint32_t wa = s < 2 ? now.w[r].x : now.w[r].y, wb = s < 2 ? now.w[r].z : now.w[r].w;
+          const int i = (s & 1) * 2;
+          const uint32_t f[4] = {weights2<PAIR>(wa, i), weights2<PAIR>(wb, i), weights2<PAIR>(wa, i + 1), weights2<PAIR>(wb, i + 1)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) mma16<PAIR>(d[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], s + p == 0 ? base[t] : d[t]);
+        }
+        const float sa = __uint_as_float((uint32_t)now.s[r][0] << 16), sb = __uint_as_float((uint32_t)now.s[r][1] << 16);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][t][e] = fmaf(PAIR ? d[t][e] * back[t][e & 1] : d[t][e], e < 2 ? sa : sb, acc[r][t][e]);
+      }
+      now = next;
     }
-  }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
+      if (r < tiles)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[warp][r * 16 + g + (e < 2 ? 0 : 8)][t * 8 + 2 * c + (e & 1)] = acc[r][t][e];
-  __syncthreads();
-  for (int i = tid; i < R * 16 * a.m; i += THREADS) {
-    const int tok = i / (R * 16), o = i - tok * (R * 16), n = t0 * 16 + o;
-    if (n >= a.n) continue;
-    float v = a.bias ? to_f32(((const T*)a.bias)[n]) : 0.f;
+          for (int e = 0; e < 4; ++e) sums[(warp * R * 16 + r * 16 + g + (e < 2 ? 0 : 8)) * LD + t * 8 + 2 * c + (e & 1)] = acc[r][t][e];
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < tiles * 16 * a.m; i += THREADS) {
+      const int tok = i / (tiles * 16), o = i - tok * (tiles * 16), n = t0 * 16 + o;
+      if (n >= a.n) continue;
+      float v = a.bias ? to_f32(((const T*)a.bias)[n]) : 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) v += sums[w][o][tok];
-    ((T*)a.out)[(size_t)tok * a.out_row + n] = from_f32<T>(v);
+      for (int w = 0; w < WARPS; ++w) v += sums[(w * R * 16 + o) * LD + tok];
+      ((T*)a.out)[tok * a.out_row + n] = from_f32<T>(v);
+    }
+    __syncthreads();
   }
 }
+
+constexpr int THREADS = 256;  // of the quantiser
 
 // One thread for 16 inputs of one output; the threads of a group are neighbours in a warp.
 template <typename T>
@@ -218,22 +256,38 @@ __global__ void __launch_bounds__(THREADS) quantize_q4_kernel(const T* w, int64_
   *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
 }
 
-template <typename T, int NT, int R>
-cudaError_t run(const Q4Args& a, cudaStream_t s) {
-  return launch_kernel(linear_q4_kernel<T, NT, R>, dim3(((a.n + 15) / 16 + R - 1) / R), dim3(THREADS), 0, s, false, a);
+template <typename T, int NT, int WARPS, int R>
+struct Variant {
+  static constexpr int SMEM = WARPS * R * 16 * (NT * 8 + 1) * 4;
+  static cudaError_t allow() { return cudaFuncSetAttribute(linear_q4_kernel<T, NT, WARPS, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); }
+  static cudaError_t run(const Q4Args& a, int sms, cudaStream_t s) {
+    return launch_kernel(linear_q4_kernel<T, NT, WARPS, R>, dim3(std::min((a.n + 15) / 16, sms)), dim3(WARPS * 32), SMEM, s, true, a);
+  }
+};
+// Few tiles for a CTA: 16 warps share the inputs' length, which is latency. Many: 8 warps with more tiles each.
+template <typename T, int NT>
+cudaError_t run_of(const Q4Args& a, int sms, cudaStream_t s) {
+  constexpr bool PAIR = std::is_same<T, float>::value;
+  return (a.n + 15) / 16 <= 3 * sms ? Variant<T, NT, 16, PAIR ? 2 : 3>::run(a, sms, s) : Variant<T, NT, 8, PAIR && NT == 2 ? 6 : 8>::run(a, sms, s);
 }
-template <typename T>
-cudaError_t run_of(const Q4Args& a, cudaStream_t s) {
-  return a.m <= 8 ? run<T, 1, 1>(a, s) : run<T, 2, 1>(a, s);
+template <typename T, int NT>
+cudaError_t allow_of() {
+  constexpr bool PAIR = std::is_same<T, float>::value;
+  const cudaError_t e = Variant<T, NT, 16, PAIR ? 2 : 3>::allow();
+  return e != cudaSuccess ? e : Variant<T, NT, 8, PAIR && NT == 2 ? 6 : 8>::allow();
 }
 
 }  // namespace
 
-cudaError_t init_q4_attributes() { return cudaSuccess; }
+cudaError_t init_q4_attributes() {
+  for (cudaError_t e : {allow_of<float, 1>(), allow_of<float, 2>(), allow_of<__nv_bfloat16, 1>(), allow_of<__nv_bfloat16, 2>()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
+}
 
 cudaError_t launch_linear_q4(const Q4Args& a, int dtype, int sms, cudaStream_t s) {
-  (void)sms;
-  return dtype == PG_DTYPE_F32 ? run_of<float>(a, s) : run_of<__nv_bfloat16>(a, s);
+  if (dtype == PG_DTYPE_F32) return a.m <= 8 ? run_of<float, 1>(a, sms, s) : run_of<float, 2>(a, sms, s);
+  return a.m <= 8 ? run_of<__nv_bfloat16, 1>(a, sms, s) : run_of<__nv_bfloat16, 2>(a, sms, s);
 }
 
 cudaError_t launch_quantize_q4(const void* w, int64_t w_row, int dtype, int n, int k, int group, uint8_t* packed, uint16_t* scales, cudaStream_t s) {
