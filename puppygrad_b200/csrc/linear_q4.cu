@@ -51,9 +51,9 @@ struct Raw {
   uint4 v[sizeof(T)];
   __device__ __forceinline__ void load(const T* p, int live, bool wide) {
     constexpr int N = 16 / sizeof(T);
-    if (wide && live >= 16) {
+    if (live <= 0 || (wide && live >= 16)) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T); ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * N);
+      for (int i = 0; i < (int)sizeof(T); ++i) v[i] = live > 0 ? *reinterpret_cast<const uint4*>(p + i * N) : make_uint4(0, 0, 0, 0);
     } else {
       union {
         uint4 u[sizeof(T)];
@@ -107,15 +107,64 @@ struct Operand<float> {
   }
 };
 
+// 64 inputs of NT groups of 8 tokens as the column operand, and what the accumulators start from.
+template <typename T, int NT>
+struct Tokens {
+  static constexpr bool PAIR = std::is_same<T, float>::value;
+  static constexpr int PARTS = PAIR ? 2 : 1;
+  Operand<T> x[NT];
+  float base[NT][4], back[NT][2];
+  __device__ __forceinline__ Tokens(const Raw<T> (&raw)[NT], int c) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float b = x[t].make(raw[t]);
+      if (PAIR) {  // columns 2 c and 2 c + 1 are the tokens of lanes 8 c and 8 c + 4
+        back[t][0] = __shfl_sync(ALL_LANES, b, c * 8);
+        back[t][1] = __shfl_sync(ALL_LANES, b, c * 8 + 4);
+      }
+      const uint32_t even = PAIR ? 0x80088008u : 0xC308C308u, odd = PAIR ? 0x80808080u : 0xC308C308u;  // -8 in either place; -136
+      const uint32_t f[4] = {even, even, odd, odd};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) base[t][e] = 0.f;
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) mma16<PAIR>(base[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
+    }
+  }
+  // 16 outputs: this lane's codes, the scales of outputs g and g + 8.
+  __device__ __forceinline__ void add(const uint4& w, uint16_t scale_a, uint16_t scale_b, float (&acc)[NT][4]) const {
+    float d[NT][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      // inputs 4 s .. 4 s + 3 of outputs g (words x, y) and g + 8 (z, w)
+      const uint32_t wa = s < 2 ? w.x : w.y, wb = s < 2 ? w.z : w.w;
+      const int i = (s & 1) * 2;
+      const uint32_t f[4] = {weights2<PAIR>(wa, i), weights2<PAIR>(wb, i), weights2<PAIR>(wa, i + 1), weights2<PAIR>(wb, i + 1)};
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          if (s + p == 0) mma16<PAIR>(d[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
+          else mma16<PAIR>(d[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], d[t]);
+        }
+    }
+    const float sa = __uint_as_float((uint32_t)scale_a << 16), sb = __uint_as_float((uint32_t)scale_b << 16);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(PAIR ? d[t][e] * back[t][e & 1] : d[t][e], e < 2 ? sa : sb, acc[t][e]);
+  }
+};
+
 // NT: groups of 8 tokens. R: tiles of 16 outputs of a pass.
 template <typename T, int NT, int WARPS, int R>
 __global__ void __launch_bounds__(WARPS * 32, 1) linear_q4_kernel(Q4Args a) {
-  constexpr bool PAIR = std::is_same<T, float>::value;
-  constexpr int THREADS = WARPS * 32, PARTS = PAIR ? 2 : 1, LD = NT * 8 + 1;
+  constexpr int THREADS = WARPS * 32, LD = NT * 8 + 1;
   extern __shared__ float sums[];  // [WARPS][R * 16][LD]
   grid_dep_launch();
   grid_dep_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int tid = threadIdx.x, warp = __shfl_sync(ALL_LANES, tid >> 5, 0), lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int row_tiles = (a.n + 15) >> 4, k_tiles = (a.k + 63) >> 6, ld = row_tiles * 16, shift = a.group == 128 ? 1 : 0;
   // this CTA's tiles, cut into passes of nearly equal size
   const int each = row_tiles / gridDim.x, more = row_tiles - each * gridDim.x;
@@ -129,14 +178,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear_q4_kernel(Q4Args a) {
     Raw<T> x[NT];
   };
   auto load = [&](Loads& l, int t0, int kt) {
-    const uint4* w = reinterpret_cast<const uint4*>(a.packed + ((size_t)t0 * k_tiles + kt) * 512) + lane;
-    const uint16_t* s = a.scales + (size_t)(kt >> shift) * ld + t0 * 16 + g;
+    // (the same for all lanes but the last term, which keeps the addresses in uniform registers)
+    const uint8_t* w = a.packed + ((int64_t)t0 * k_tiles + kt) * 512;
+    const uint16_t* s = a.scales + (int64_t)(kt >> shift) * ld + t0 * 16;
+    const int tiles = min(per_pass, t_first + t_count - t0);
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (r == 0 || (r < per_pass && t0 + r < t_first + t_count)) {
-        l.w[r] = __ldg(w + (size_t)r * k_tiles * 32);
-        l.s[r][0] = __ldg(s + r * 16);
-        l.s[r][1] = __ldg(s + r * 16 + 8);
+      if (r == 0 || r < tiles) {
+        l.w[r] = __ldg(reinterpret_cast<const uint4*>(w + (int64_t)r * k_tiles * 512) + lane);
+        l.s[r][0] = __ldg(s + r * 16 + g);
+        l.s[r][1] = __ldg(s + r * 16 + 8 + g);
       }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -156,50 +207,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear_q4_kernel(Q4Args a) {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[r][t][e] = 0.f;
+    auto add = [&](const Loads& l) {
+      const Tokens<T, NT> x(l.x, c);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r == 0 || r < tiles) x.add(l.w[r], l.s[r][0], l.s[r][1], acc[r]);
+    };
 #pragma unroll 1
     for (int kt = warp; kt < k_tiles; kt += WARPS) {
       // the next tile of inputs, or the next pass's first one
       if (kt + WARPS < k_tiles) load(next, t0, kt + WARPS);
       else if (t0 + per_pass < t_first + t_count) load(next, t0 + per_pass, warp);
-      Operand<T> x[NT];
-      float base[NT][4], back[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float b = x[t].make(now.x[t]);
-        if (PAIR) {  // columns 2 c and 2 c + 1 are the tokens of lanes 8 c and 8 c + 4
-          back[t][0] = __shfl_sync(ALL_LANES, b, c * 8);
-          back[t][1] = __shfl_sync(ALL_LANES, b, c * 8 + 4);
-        }
-        const uint32_t even = PAIR ? 0x80088008u : 0xC308C308u, odd = PAIR ? 0x80808080u : 0xC308C308u;  // -8 in either place; -136
-        const uint32_t f[4] = {even, even, odd, odd};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) base[t][e] = 0.f;
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-          for (int s = 0; s < 4; ++s) mma16<PAIR>(base[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r > 0 && r >= tiles) continue;
-        float d[NT][4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          // inputs 4 s .. 4 s + 3 of outputs g (words x, y) and g + 8 (z, w)
-          const uint32_t wa = s < 2 ? now.w[r].x : now.w[r].y, wb = s < 2 ? now.w[r].z : now.w[r].w;
-          const int i = (s & 1) * 2;
-          const uint32_t f[4] = {weights2<PAIR>(wa, i), weights2<PAIR>(wb, i), weights2<PAIR>(wa, i + 1), weights2<PAIR>(wb, i + 1)};
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) mma16<PAIR>(d[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], s + p == 0 ? base[t] : d[t]);
-        }
-        const float sa = __uint_as_float((uint32_t)now.s[r][0] << 16), sb = __uint_as_float((uint32_t)now.s[r][1] << 16);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[r][t][e] = fmaf(PAIR ? d[t][e] * back[t][e & 1] : d[t][e], e < 2 ? sa : sb, acc[r][t][e]);
-      }
+      add(now);
       now = next;
     }
 #pragma unroll
@@ -264,30 +283,31 @@ struct Variant {
     return launch_kernel(linear_q4_kernel<T, NT, WARPS, R>, dim3(std::min((a.n + 15) / 16, sms)), dim3(WARPS * 32), SMEM, s, true, a);
   }
 };
-// Few tiles for a CTA: 16 warps share the inputs' length, which is latency. Many: 8 warps with more tiles each.
+// Few tiles of outputs for a CTA: 16 warps share the inputs' length, which is latency. Many: 8 warps, whose registers hold more tiles, so
+// that what is done once for 64 inputs serves more outputs.
 template <typename T, int NT>
-cudaError_t run_of(const Q4Args& a, int sms, cudaStream_t s) {
-  constexpr bool PAIR = std::is_same<T, float>::value;
-  return (a.n + 15) / 16 <= 3 * sms ? Variant<T, NT, 16, PAIR ? 2 : 3>::run(a, sms, s) : Variant<T, NT, 8, PAIR && NT == 2 ? 6 : 8>::run(a, sms, s);
-}
-template <typename T, int NT>
-cudaError_t allow_of() {
-  constexpr bool PAIR = std::is_same<T, float>::value;
-  const cudaError_t e = Variant<T, NT, 16, PAIR ? 2 : 3>::allow();
-  return e != cudaSuccess ? e : Variant<T, NT, 8, PAIR && NT == 2 ? 6 : 8>::allow();
-}
+struct Choice {
+  static constexpr bool PAIR = std::is_same<T, float>::value;
+  using Few = Variant<T, NT, PAIR && NT == 2 ? 8 : 16, PAIR ? 2 : 3>;
+  using Many = Variant<T, NT, 8, 8>;
+  static cudaError_t run(const Q4Args& a, int sms, cudaStream_t s) { return (a.n + 15) / 16 <= 3 * sms ? Few::run(a, sms, s) : Many::run(a, sms, s); }
+  static cudaError_t allow() {
+    const cudaError_t e = Few::allow();
+    return e != cudaSuccess ? e : Many::allow();
+  }
+};
 
 }  // namespace
 
 cudaError_t init_q4_attributes() {
-  for (cudaError_t e : {allow_of<float, 1>(), allow_of<float, 2>(), allow_of<__nv_bfloat16, 1>(), allow_of<__nv_bfloat16, 2>()})
+  for (cudaError_t e : {Choice<float, 1>::allow(), Choice<float, 2>::allow(), Choice<__nv_bfloat16, 1>::allow(), Choice<__nv_bfloat16, 2>::allow()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
 
 cudaError_t launch_linear_q4(const Q4Args& a, int dtype, int sms, cudaStream_t s) {
-  if (dtype == PG_DTYPE_F32) return a.m <= 8 ? run_of<float, 1>(a, sms, s) : run_of<float, 2>(a, sms, s);
-  return a.m <= 8 ? run_of<__nv_bfloat16, 1>(a, sms, s) : run_of<__nv_bfloat16, 2>(a, sms, s);
+  if (dtype == PG_DTYPE_F32) return a.m <= 8 ? Choice<float, 1>::run(a, sms, s) : Choice<float, 2>::run(a, sms, s);
+  return a.m <= 8 ? Choice<__nv_bfloat16, 1>::run(a, sms, s) : Choice<__nv_bfloat16, 2>::run(a, sms, s);
 }
 
 cudaError_t launch_quantize_q4(const void* w, int64_t w_row, int dtype, int n, int k, int group, uint8_t* packed, uint16_t* scales, cudaStream_t s) {

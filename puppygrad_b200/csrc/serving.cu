@@ -214,8 +214,7 @@ static int check_q4(const void* packed, const void* scales, int n, int k, int gr
   if (n < 1 || k < 1 || n > (1 << 28) || k > (1 << 28)) return bad("n and k must be in 1..2^28");
   if (group != 64 && group != 128) return bad("group " + std::to_string(group) + " must be 64 or 128");
   if (!packed || !scales) return bad("packed or scales is null");
-  if (!aligned(packed, 16)) return bad("packed is not 16-byte aligned");
-  if (!aligned(scales, 2)) return bad("scales is not aligned to its type");
+  if (!aligned(packed, 16) || !aligned(scales, 16)) return bad("packed or scales is not 16-byte aligned");
   return PG_OK;
 }
 

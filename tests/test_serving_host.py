@@ -74,7 +74,7 @@ def test_attention_is_checked(kw, text):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(m=0), "m 0 must be in 1..16"), (dict(m=17), "m 17"), (dict(n=0), "n and k"), (dict(k=0), "n and k"), (dict(group=32), "group 32"), (dict(p=0), "packed or scales"),
-    (dict(s=0), "packed or scales"), (dict(p=P + 8), "16-byte aligned"), (dict(xs=63), "x: distance"), (dict(os=15), "out: distance"), (dict(dtype=-1), "dtype -1"),
+    (dict(s=0), "packed or scales"), (dict(p=P + 8), "16-byte aligned"), (dict(s=P + 8), "16-byte aligned"), (dict(xs=63), "x: distance"), (dict(os=15), "out: distance"), (dict(dtype=-1), "dtype -1"),
     (dict(b=P + 2), "bias"), (dict(x=P + 1, dtype=1), "x is not aligned"),
 ])
 def test_linear_q4_is_checked(kw, text):
