@@ -466,7 +466,7 @@ def check_scores(x, targets, top):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (2, 7, 7), (3, 33, 32), (1, 50257, 5), (8, 50257, 20), (200, 1000, 1), (149, 5003, 32), (5, 128256, 8), (600, 2049, 0),
-                                            (1, 1000003, 32), (40, 40, 32)])
+                                            (1, 1000003, 32), (40, 40, 32), (2000, 777, 3), (1800, 5000, 32), (500, 3001, 20)])
 def test_token_logprobs(rows, vocab, top, dtype):
     g = gen(rows + vocab)
     x = (torch.randn(rows, vocab + 3, generator=g, device=DEV) * 3).to(dtype)[:, 1:vocab + 1]  # rows at odd addresses
@@ -478,8 +478,9 @@ def test_token_logprobs(rows, vocab, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("repeat", [1, 60, 200])
 @pytest.mark.parametrize("vocab", [5, 600, 50257])
-def test_token_logprobs_masks_and_ties(dtype, vocab):
+def test_token_logprobs_masks_and_ties(dtype, vocab, repeat):
     """Ties go to the lower id, masked entries have no weight, rows of one kind of value work."""
     low = torch.finfo(dtype).min
     x = torch.zeros(10, vocab, device=DEV, dtype=dtype)  # row 0: all equal
@@ -495,18 +496,26 @@ def test_token_logprobs_masks_and_ties(dtype, vocab):
     x[8] = torch.finfo(dtype).max
     x[9, -1] = 3e38
     top = min(5, vocab)
+    x = x.repeat(repeat, 1) if vocab < 50257 else x
     t = torch.tensor([0, vocab - 2, 1, 2, vocab - 1, 0, 1, 0, 3, vocab - 1], dtype=torch.int32, device=DEV)
-    check_scores(x, t, top)
+    check_scores(x, t.repeat(x.shape[0] // 10), top)
 
 
-def test_token_logprobs_rows_without_a_distribution_and_odd_targets():
+@pytest.mark.parametrize("offset", [1000.0, -30000.0])
+def test_token_logprobs_of_logits_far_from_zero(offset):
+    x = torch.randn(20, 5000, generator=gen(1), device=DEV) + offset
+    check_scores(x, torch.arange(20, dtype=torch.int32, device=DEV), 5)
+
+
+@pytest.mark.parametrize("repeat", [1, 100, 400])  # a block, four warps, a warp for each row
+def test_token_logprobs_rows_without_a_distribution_and_odd_targets(repeat):
     for vocab in (9, 3000, 50257):
         x = torch.randn(6, vocab, device=DEV)
         x[1, vocab - 1] = math.nan
         x[2, 0] = math.inf
         x[3] = -math.inf
         t = torch.tensor([-1, 0, 0, 0, vocab, -2], dtype=torch.int32, device=DEV)
-        lp, ent, ids, values = run_scores(x, t, 3)
+        lp, ent, ids, values = (o[-6:] for o in run_scores(x.repeat(repeat, 1), t.repeat(repeat), 3))
         assert lp[0] == 0 and torch.isnan(lp[1:]).all()
         assert torch.isnan(ent[1:4]).all() and torch.isfinite(ent[[0, 4, 5]]).all()
         assert (ids[1:4] == -1).all() and torch.isnan(values[1:4]).all() and (ids[[0, 4, 5]] >= 0).all()
