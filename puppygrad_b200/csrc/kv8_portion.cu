@@ -1,18 +1,19 @@
 // Attention over the 8-bit paged cache for sequences with many new rows: portions of prompts.
 //
-// A CTA has a tile of 128 (token, query head of the group) rows that share a key / value head, and walks the pieces of 64 positions
-// that any of them sees. Both products are tcgen05 instructions on FP16 operands: S = Q K^T with both in shared memory, O += P V with
-// P in tensor memory in the place of S and O in tensor memory. Four producer warps load codes (sent for one piece ahead, in
-// registers), turn them into FP16 (exact) and store them with the operands' 128-byte swizzle: keys lie by token, values by
-// head entry, so both are K-major as they come. Four softmax warps have a row for every thread, which needs no exchange between
+// A CTA has one or two tiles of 128 (token, query head of the group) rows that share a key / value head, and walks the pieces of 64
+// positions that any of them sees. Both products are tcgen05 instructions on FP16 operands: S = Q K^T with both in shared memory, O += P V
+// with P in tensor memory in the place of S and O in tensor memory. Four producer warps load codes (sent for one piece ahead, in
+// registers), turn them into FP16 (exact) and store them with the operands' 128-byte swizzle: keys lie by token, values by head entry,
+// so both are K-major as they come. Four softmax warps for each tile have a row for every thread, which needs no exchange between
 // threads; one warp issues the products, the scores of a piece in front of the values of the one before it, so that the tensor pipe
-// works while the softmax of the next scores is computed. Two CTAs share an SM up to head_dim 128 (FP32: 64).
+// works while the softmax of the next scores is computed. Two tiles (head_dim up to 128: tensor memory holds both) share the
+// producers' work, and one's softmax runs beside the other's products.
 //
 // Scales, weights and the running maximum are those of the step kernel: the value scale is part of the exponent, the denominator
 // divides it out. The maximum that weights refer to moves only when a row outgrows it by 2^8 (FP16 holds 2^15), which spares most
 // passes over O. FP32 rows are pairs of FP16 numbers, queries and weights alike: two products into the same accumulator.
-// Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe about equally
-// busy at head_dim 128.
+// Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy
+// at head_dim 128, 1024 cycles for 256 rows and 64 positions.
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -21,17 +22,18 @@
 namespace pg {
 namespace {
 
-constexpr int ROWS = 128, TOKENS = 64, SOFTMAX_WARPS = 4, PRODUCER_WARPS = 4, THREADS = (SOFTMAX_WARPS + 1 + PRODUCER_WARPS) * 32;
+constexpr int ROWS = 128, TOKENS = 64, TILE_WARPS = 4, PRODUCER_WARPS = 4;
 
 template <int DP, typename T>
 struct PortionShape {
   static constexpr bool PAIR = std::is_same<T, float>::value;
-  static constexpr int KC = DP / 64;
-  static constexpr int QUERIES = (PAIR ? 2 : 1) * KC * 16384, HALF = KC * 8192, STAGE = 2 * HALF;  // bytes
-  static constexpr int STAGES = PAIR && DP == 256 ? 1 : 2;
+  static constexpr int KC = DP / 64, TILES = DP <= 128 ? 2 : 1;
+  static constexpr int SOFTMAX_WARPS = TILES * TILE_WARPS, THREADS = (SOFTMAX_WARPS + 1 + PRODUCER_WARPS) * 32;
+  static constexpr int TILE_QUERIES = (PAIR ? 2 : 1) * KC * 16384, QUERIES = TILES * TILE_QUERIES, HALF = KC * 8192, STAGE = 2 * HALF;  // bytes
+  static constexpr int STAGES = QUERIES + 3 * STAGE <= 192 * 1024 ? 3 : QUERIES + 2 * STAGE <= 192 * 1024 ? 2 : 1;
   static constexpr int SMEM = QUERIES + STAGES * STAGE + 1024;
-  static constexpr int COLS = DP + 128 <= 256 ? 256 : 512;  // tensor memory: O, then two places for scores and weights
-  static constexpr int CTAS = COLS == 256 && SMEM <= 113 * 1024 ? 2 : 1;
+  static constexpr int COLS = 512;  // tensor memory: for each tile O, then two places for scores and weights
+  static_assert(TILES * (DP + 128) <= COLS, "tensor memory");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -44,18 +46,38 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// 64 columns of this warp's 32 rows.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[4][16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_ld16_issue(taddr + i * 16, r[i]);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i >> 4][i & 15]);
+}
+__device__ __forceinline__ unsigned long long add_two(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <int DP, typename T>
-__global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portion_kernel(Kv8AttnArgs a, int slots) {
+__global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_kernel(Kv8AttnArgs a, int slots) {
   using S = PortionShape<DP, T>;
   constexpr bool PAIR = S::PAIR;
-  constexpr int KC = S::KC, STAGES = S::STAGES, ITEMS = DP / 32;  // 16-byte items of keys (and of values) for every producer thread
+  constexpr int KC = S::KC, STAGES = S::STAGES, TILES = S::TILES, SOFTMAX_WARPS = S::SOFTMAX_WARPS;
+  constexpr int ITEMS = DP / 32;  // 16-byte items of keys (and of values) for every producer thread
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, full[2], empty[2], s_full[2], p_full, o_done;
+  __shared__ uint64_t q_full[TILES], full[STAGES], empty[STAGES], s_full[TILES][2], p_full[TILES][2], o_done[TILES];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_flag;
-  __shared__ float4 info[2][3];  // of a stage's four pieces of 16 tokens: key scale, log2 of the value scale, its inverse
+  __shared__ float4 info[STAGES][3];  // of a stage's four pieces of 16 tokens: key scale, log2 of the value scale, its inverse
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* stages = base + S::QUERIES;
   volatile int* failed = &failed_flag;
@@ -64,9 +86,9 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
   grid_dep_launch();
   grid_dep_wait();
 
-  // ---- the tile: slots of a sequence begin at floor(first row * group / ROWS) + b; the longest rows of a sequence first
+  // ---- the tile: slots of a sequence begin at floor(first row * group / its rows) + b; the longest rows of a sequence first
   const int slot = slots - 1 - (int)(blockIdx.x / c.kv_heads), head = blockIdx.x % c.kv_heads;
-  auto first_slot = [&](int s) { return (int)((int64_t)min(max(a.row_start[s], 0), a.rows) * a.group / ROWS) + s; };
+  auto first_slot = [&](int s) { return (int)((int64_t)min(max(a.row_start[s], 0), a.rows) * a.group / (TILES * ROWS)) + s; };
   int lo = 0, hi = c.seqs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -75,24 +97,29 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
   }
   const int b = lo;
   const SeqRows r = seq_rows(a.row_start, a.rows, b);
-  const int row0 = (slot - first_slot(b)) * ROWS, rows = min(ROWS, r.n * a.group - row0);
+  const int row0 = (slot - first_slot(b)) * (TILES * ROWS), rows = min(TILES * ROWS, r.n * a.group - row0);
   if (row0 < 0 || rows <= 0 || r.n * a.group <= a.step_rows) return;  // few rows: the step kernel's
   const int len = max(a.lens[b], 0), have = min(len, c.pages_per_seq << c.page_shift);
   const int pos_low = len - r.n + row0 / a.group, pos_high = len - r.n + (row0 + rows - 1) / a.group;
   const int high = (max(min(pos_high + 1, have), 0) + TOKENS - 1) / TOKENS;
   const int low = a.window > 0 ? min(max(pos_low - a.window + 1, 0) / TOKENS, high) : 0;
-  const int kept = min((min(a.keep, have) + TOKENS - 1) / TOKENS, low), tiles = kept + high - low;
+  const int kept = min((min(a.keep, have) + TOKENS - 1) / TOKENS, low), pieces = kept + high - low;
+  const int tiles = rows > ROWS ? TILES : 1;  // that have rows
   auto start_of = [&](int j) { return (j < kept ? j : low + j - kept) * TOKENS; };
 
   if (tid == 0) {
-    mbar_init(&q_full, SOFTMAX_WARPS);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], PRODUCER_WARPS);
       mbar_init(&empty[i], 1);
-      mbar_init(&s_full[i], 1);
     }
-    mbar_init(&p_full, SOFTMAX_WARPS);
-    mbar_init(&o_done, 1);
+    for (int i = 0; i < TILES; ++i) {
+      mbar_init(&q_full[i], TILE_WARPS);
+      mbar_init(&s_full[i][0], 1);
+      mbar_init(&s_full[i][1], 1);
+      mbar_init(&p_full[i][0], TILE_WARPS);
+      mbar_init(&p_full[i][1], TILE_WARPS);
+      mbar_init(&o_done[i], 1);
+    }
     failed_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -100,135 +127,154 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot, tmem_s = tmem + DP;
+  const uint32_t tmem = tmem_slot;
+  auto o_of = [&](int t) { return tmem + (uint32_t)(t * (DP + 128)); };
   bool ok = true;
 
   if (warp < SOFTMAX_WARPS) {
     // ---- a row for every thread
-    const int i = tid, x = row0 + min(i, rows - 1), tok = x / a.group, g = x - tok * a.group;
+    const int tile = warp / TILE_WARPS, in_tile = tid & (ROWS - 1);
+    const bool used = tile < tiles;
+    const int i = tile * ROWS + in_tile, x = row0 + min(i, rows - 1), tok = x / a.group, g = x - tok * a.group;
     const int pos = len - r.n + tok;
-    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    const T* q = (const T*)a.q + (size_t)(r.first + tok) * a.q_row + (size_t)(head * a.group + g) * c.dim;
-    const bool wide = c.dim % 8 == 0 && ((uintptr_t)q & 15) == 0;
-    auto eight = [&](int d, float (&v)[8]) {
-      if (wide && d + 8 <= c.dim) {
-        load8(q + d, v);
-      } else {
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tmem_o = o_of(tile) + lane_addr, tmem_s = tmem_o + DP;
+    float back = 0.f;
+    if (used) {
+      const T* q = (const T*)a.q + (size_t)(r.first + tok) * a.q_row + (size_t)(head * a.group + g) * c.dim;
+      const bool wide = c.dim % 8 == 0 && ((uintptr_t)q & 15) == 0;
+      auto eight = [&](int d, float (&v)[8]) {
+        if (wide && d + 8 <= c.dim) {
+          load8(q + d, v);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = d + e < c.dim ? to_f32(q[d + e]) : 0.f;
+          for (int e = 0; e < 8; ++e) v[e] = d + e < c.dim ? to_f32(q[d + e]) : 0.f;
+        }
+      };
+      float top = 0.f;
+      for (int d = 0; d < c.dim; d += 8) {
+        float v[8];
+        eight(d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
       }
-    };
-    float top = 0.f;
-    for (int d = 0; d < c.dim; d += 8) {
-      float v[8];
-      eight(d, v);
+      // the sign of the score's factor goes to the queries, so that the largest product is the largest score
+      const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const float f = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), a.scale);
+      back = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23), 1e-37f);  // never 0: a masked score is infinite
+      for (int u = 0; u < DP / 8; ++u) {  // 16 bytes each
+        float v[8];
+        eight(u * 8, v);
+        uint8_t* to = base + tile * S::TILE_QUERIES + (u >> 3) * 16384 + in_tile * 128 + (((u & 7) ^ (in_tile & 7)) << 4);
+        uint32_t h[4], l[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-    }
-    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
-    const float f = __uint_as_float((uint32_t)(127 - ex) << 23), back = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23);
-    for (int u = 0; u < DP / 8; ++u) {  // 16 bytes each
-      float v[8];
-      eight(u * 8, v);
-      uint8_t* to = base + (u >> 3) * 16384 + i * 128 + (((u & 7) ^ (i & 7)) << 4);
-      uint32_t h[4], l[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        h[e] = pack_f16(v[2 * e] * f, v[2 * e + 1] * f);
-        const float2 p = unpack_f16(h[e]);
-        l[e] = pack_f16(v[2 * e] * f - p.x, v[2 * e + 1] * f - p.y);
+        for (int e = 0; e < 4; ++e) {
+          h[e] = pack_f16(v[2 * e] * f, v[2 * e + 1] * f);
+          const float2 p = unpack_f16(h[e]);
+          l[e] = pack_f16(v[2 * e] * f - p.x, v[2 * e + 1] * f - p.y);
+        }
+        *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (PAIR) *reinterpret_cast<uint4*>(to + KC * 16384) = make_uint4(l[0], l[1], l[2], l[3]);
       }
-      *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-      if (PAIR) *reinterpret_cast<uint4*>(to + KC * 16384) = make_uint4(l[0], l[1], l[2], l[3]);
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[tile]);
     }
-    fence_async_proxy();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&q_full);
 
     float m_ref = -INFINITY, sum = 0.f;
-    for (int j = 0; j < tiles; ++j) {
-      const uint32_t s_at = tmem_s + (uint32_t)(j & 1) * 64 + lane_addr;
-      ok = __all_sync(ALL_LANES, ok && mbar_wait(&s_full[j & 1], (j >> 1) & 1, failed, nullptr, 0));
+    int stage = 0;
+    for (int j = 0; j < pieces && used; ++j) {
+      const uint32_t s_at = tmem_s + (uint32_t)(j & 1) * 64;
+      ok = __all_sync(ALL_LANES, ok && mbar_wait(&s_full[tile][j & 1], (j >> 1) & 1, failed, nullptr, 0));
       if (!ok) break;
       tc_fence_after();
       const int t0 = start_of(j);
-      const float4 k4 = info[j % STAGES][0], e4 = info[j % STAGES][1], i4 = info[j % STAGES][2];
-      const float kf[4] = {k4.x * back, k4.y * back, k4.z * back, k4.w * back}, ev[4] = {e4.x, e4.y, e4.z, e4.w}, inv[4] = {i4.x, i4.y, i4.z, i4.w};
-      const bool whole = t0 + TOKENS - 1 <= pos_low && t0 + TOKENS <= have && (a.window == 0 || t0 > pos_high - a.window || t0 + TOKENS <= a.keep);
-      const int hi_i = min(pos, have - 1) - t0, lo_i = a.window > 0 ? pos - a.window + 1 - t0 : -1, keep_i = a.keep - t0;
-      auto exponents = [&](int h, float (&v)[32]) {
-        tmem_ld32(s_at + h * 32, v);
+      const float4 k4 = info[stage][0], e4 = info[stage][1], i4 = info[stage][2];
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      float kf[4] = {k4.x * back, k4.y * back, k4.z * back, k4.w * back}, ev[4] = {e4.x, e4.y, e4.z, e4.w};
+      const float inv[4] = {i4.x, i4.y, i4.z, i4.w};
+      float v[64];
+      tmem_ld64(s_at, v);
+      if (!(t0 + TOKENS - 1 <= pos_low && t0 + TOKENS <= have && (a.window == 0 || t0 > pos_high - a.window || t0 + TOKENS <= a.keep))) {
+        const int hi_i = min(pos, have - 1) - t0, lo_i = a.window > 0 ? pos - a.window + 1 - t0 : -1, keep_i = a.keep - t0;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], kf[h * 2 + e / 16], ev[h * 2 + e / 16]);
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (h * 32 + e > hi_i || (h * 32 + e < lo_i && h * 32 + e >= keep_i)) v[e] = -INFINITY;
+        for (int e = 0; e < 64; ++e) {
+          const bool hidden = e > hi_i || (e < lo_i && e >= keep_i);
+          v[e] = hidden ? -INFINITY : fmaf(v[e], kf[e / 16], ev[e / 16]);  // whatever the scales are
         }
-      };
-      float tile_top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        exponents(h, v);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) tile_top[e & 3] = fmaxf(tile_top[e & 3], v[e]);
+        for (int h = 0; h < 4; ++h) kf[h] = 1.f, ev[h] = 0.f;
       }
-      const float t_max = fmaxf(fmaxf(tile_top[0], tile_top[1]), fmaxf(tile_top[2], tile_top[3]));
-      if (__any_sync(ALL_LANES, t_max > m_ref + 8.f || (m_ref == -INFINITY && t_max > -INFINITY))) {
+      float t_max = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float m = fmaxf(v[h * 16], v[h * 16 + 1]);
+#pragma unroll
+        for (int e = 2; e < 16; e += 2) m = fmaxf(m, fmaxf(v[h * 16 + e], v[h * 16 + e + 1]));
+        t_max = fmaxf(t_max, fmaf(m, kf[h], ev[h]));
+      }
+      if (__any_sync(ALL_LANES, t_max > m_ref + 8.f)) {
         const float m_new = fmaxf(m_ref, t_max), corr = m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new);
         m_ref = m_new;
         sum *= corr;
         if (j > 0) {
-          ok = __all_sync(ALL_LANES, mbar_wait(&o_done, (j - 1) & 1, failed, nullptr, 0));
+          ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (j - 1) & 1, failed, nullptr, 0));
           if (!ok) break;
           tc_fence_after();
+#pragma unroll 1
           for (int d = 0; d < DP; d += 16) {
             float o[16];
-            tmem_ld16(tmem + lane_addr + d, o);
+            tmem_ld16(tmem_o + d, o);
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * corr);
-            tmem_st16(tmem + lane_addr + d, w);
+            tmem_st16(tmem_o + d, w);
           }
         }
       }
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        exponents(h, v);
-        float part[2] = {0.f, 0.f};
-        uint32_t hi16[16], lo16[16];
+      for (int h = 0; h < 4; ++h) {
+        const float b = ev[h] - m_use;
+        const unsigned long long k2 = pack2(kf[h], kf[h]), b2 = pack2(b, b);
+        unsigned long long part = pack2(0.f, 0.f);
+        uint32_t hi16[8], lo16[8];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float p0 = ex2(v[e] - m_use), p1 = ex2(v[e + 1] - m_use);
-          part[e / 16] += p0 + p1;
+        for (int e = 0; e < 16; e += 2) {
+          float p0, p1;
+          unpack2(fma2(pack2(v[h * 16 + e], v[h * 16 + e + 1]), k2, b2), p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          part = add_two(part, pack2(p0, p1));
           hi16[e / 2] = pack_f16(p0, p1);
           if (PAIR) {
             const float2 p = unpack_f16(hi16[e / 2]);
             lo16[e / 2] = pack_f16(p0 - p.x, p1 - p.y);
           }
         }
-        sum = fmaf(part[0], inv[h * 2], fmaf(part[1], inv[h * 2 + 1], sum));
-        tmem_st16(s_at + h * 32, hi16);
-        if (PAIR) tmem_st16(s_at + h * 32 + 16, lo16);
+        float a0, a1;
+        unpack2(part, a0, a1);
+        sum = fmaf(a0 + a1, inv[h], sum);
+        // (the scores are in registers: any order of storing is fine)
+        tmem_st8(s_at + (h >> 1) * 32 + (h & 1) * 8, hi16);
+        if (PAIR) tmem_st8(s_at + (h >> 1) * 32 + 16 + (h & 1) * 8, lo16);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full);
+      if (lane == 0) mbar_arrive(&p_full[tile][j & 1]);  // (two in turn: the next one's may come before this one is waited for)
     }
-    if (ok && tiles > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done, (tiles - 1) & 1, failed, nullptr, 0));
-    if (ok) {
+    if (ok && used && pieces > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (pieces - 1) & 1, failed, nullptr, 0));
+    if (ok && used) {
       tc_fence_after();
       const float by = sum == 0.f ? 0.f : 1.f / sum;
       T* out = (T*)a.out + (size_t)(r.first + tok) * a.out_row + (size_t)(head * a.group + g) * c.dim;
       const bool wide_out = c.dim % 8 == 0 && ((uintptr_t)out & 15) == 0;
+#pragma unroll 1
       for (int d = 0; d < c.dim; d += 16) {
         float o[16];
-        if (tiles > 0) {
-          tmem_ld16(tmem + lane_addr + d, o);
+        if (pieces > 0) {
+          tmem_ld16(tmem_o + d, o);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -253,44 +299,52 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
     tc_fence_before();
   } else if (warp == SOFTMAX_WARPS) {
     // ---- products
-    if (lane == 0 && tiles > 0) {
+    if (lane == 0 && pieces > 0) {
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(TOKENS >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       const uint64_t q_desc = umma_desc_sw128(base), kv_desc = umma_desc_sw128(stages);
+      RingCursor ahead, now;  // the stage whose scores are next, and the one whose values are
       auto scores = [&](int j) {
-        if (!mbar_wait(&full[j % STAGES], (j / STAGES) & 1, failed, nullptr, 0)) return false;
+        if (!mbar_wait(&full[ahead.stage], ahead.parity, failed, nullptr, 0)) return false;
         tc_fence_after();
-        const uint64_t dk = kv_desc + (uint32_t)(j % STAGES) * (S::STAGE >> 4);
-        const uint32_t to = tmem_s + (uint32_t)(j & 1) * 64;
+        const uint64_t dk = kv_desc + ahead.stage * (S::STAGE >> 4);
+        for (int t = 0; t < tiles; ++t) {
+          const uint32_t to = o_of(t) + DP + (uint32_t)(j & 1) * 64;
+          const uint64_t dq = q_desc + (uint32_t)t * (S::TILE_QUERIES >> 4);
 #pragma unroll
-        for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+          for (int p = 0; p < (PAIR ? 2 : 1); ++p)
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            umma_bf16_ss(to, q_desc + (uint32_t)((p * KC + (k >> 2)) * (16384 >> 4) + (k & 3) * 2), dk + (uint32_t)((k >> 2) * (8192 >> 4) + (k & 3) * 2),
-                         idesc_s, (p | k) != 0);
-        umma_commit(&s_full[j & 1]);
+            for (int k = 0; k < DP / 16; ++k)
+              umma_bf16_ss(to, dq + (uint32_t)((p * KC + (k >> 2)) * (16384 >> 4) + (k & 3) * 2), dk + (uint32_t)((k >> 2) * (8192 >> 4) + (k & 3) * 2),
+                           idesc_s, (p | k) != 0);
+          umma_commit(&s_full[t][j & 1]);
+        }
+        ahead.next(STAGES);
         return true;
       };
-      ok = mbar_wait(&q_full, 0, failed, nullptr, 0);
+      for (int t = 0; t < tiles && ok; ++t) ok = mbar_wait(&q_full[t], 0, failed, nullptr, 0);
       if (ok && STAGES > 1) ok = scores(0);
-      for (int j = 0; j < tiles && ok; ++j) {
+      for (int j = 0; j < pieces && ok; ++j) {
         if (STAGES > 1) {
-          if (j + 1 < tiles) ok = scores(j + 1);
+          if (j + 1 < pieces) ok = scores(j + 1);
         } else {
           ok = scores(j);
         }
-        ok = ok && mbar_wait(&p_full, j & 1, failed, nullptr, 0);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t dv = kv_desc + (uint32_t)((j % STAGES) * (S::STAGE >> 4) + (S::HALF >> 4));
-        const uint32_t from = tmem_s + (uint32_t)(j & 1) * 64;
+        const uint64_t dv = kv_desc + (uint32_t)(now.stage * (S::STAGE >> 4) + (S::HALF >> 4));
+        for (int t = 0; t < tiles && ok; ++t) {
+          ok = mbar_wait(&p_full[t][j & 1], (j >> 1) & 1, failed, nullptr, 0);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t to = o_of(t), from = to + DP + (uint32_t)(j & 1) * 64;
 #pragma unroll
-        for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+          for (int p = 0; p < (PAIR ? 2 : 1); ++p)
 #pragma unroll
-          for (int k = 0; k < TOKENS / 16; ++k)
-            umma_bf16_ts(tmem, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (j | p | k) != 0);
-        umma_commit(&empty[j % STAGES]);
-        umma_commit(&o_done);
+            for (int k = 0; k < TOKENS / 16; ++k)
+              umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (j | p | k) != 0);
+          umma_commit(&o_done[t]);
+        }
+        if (ok) umma_commit(&empty[now.stage]);
+        now.next(STAGES);
       }
     }
     __syncwarp();
@@ -299,7 +353,7 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
     const int p_tid = tid - (SOFTMAX_WARPS + 1) * 32, mask = c.page_tokens - 1;
     const size_t block = (size_t)DP << c.page_shift;
     auto look_up = [&](int j) {  // the page of 16 tokens, of piece lane % 4
-      if (j >= tiles) return -1;
+      if (j >= pieces) return -1;
       const int tok = start_of(j) + (lane & 3) * 16;
       return tok < have ? page_of(c, b, tok >> c.page_shift) : -1;
     };
@@ -330,10 +384,11 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
       x = make_uint4(e4m3x2_to_f16x2(v.x & 0xFFFFu), e4m3x2_to_f16x2(v.x >> 16), e4m3x2_to_f16x2(v.y & 0xFFFFu), e4m3x2_to_f16x2(v.y >> 16));
       y = make_uint4(e4m3x2_to_f16x2(v.z & 0xFFFFu), e4m3x2_to_f16x2(v.z >> 16), e4m3x2_to_f16x2(v.w & 0xFFFFu), e4m3x2_to_f16x2(v.w >> 16));
     };
-    if (tiles > 0) load(0);
-    for (int j = 0; j < tiles; ++j) {
-      const int next_page = look_up(j + 1), stage = j % STAGES;
-      ok = __all_sync(ALL_LANES, ok && mbar_wait(&empty[stage], ((j / STAGES) & 1) ^ 1, failed, nullptr, 0));
+    if (pieces > 0) load(0);
+    RingCursor at;
+    for (int j = 0; j < pieces; ++j, at.next(STAGES)) {
+      const int next_page = look_up(j + 1), stage = at.stage;
+      ok = __all_sync(ALL_LANES, ok && mbar_wait(&empty[stage], at.parity ^ 1, failed, nullptr, 0));
       if (!ok) break;
       uint8_t* ks = stages + stage * S::STAGE;
       uint8_t* vs = ks + S::HALF;
@@ -366,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
         const float sv = fmaxf(scale.y, 7.888609e-31f);  // 2^-100, the least scale that an append writes
         const bool odd = scale.y != scale.y;
         float* to = reinterpret_cast<float*>(&info[stage][0]) + p_tid;
-        to[0] = scale.x;
+        to[0] = page < 0 ? 1.f : scale.x;
         to[4] = page < 0 ? -INFINITY : odd ? scale.y : __log2f(sv);
         to[8] = page < 0 || odd ? 1.f : 1.f / sv;
       }
@@ -374,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[stage]);
       page = next_page;
-      if (j + 1 < tiles) load(j + 1);
+      if (j + 1 < pieces) load(j + 1);
     }
   }
   // ---- all products are done: the softmax warps have waited for the last one, or a wait ran out, which happens to none that was issued
@@ -387,8 +442,8 @@ __global__ void __launch_bounds__(THREADS, PortionShape<DP, T>::CTAS) kv8_portio
 template <int DP, typename T>
 cudaError_t run(const Kv8AttnArgs& a, cudaStream_t s) {
   using S = PortionShape<DP, T>;
-  const int slots = (int)((int64_t)a.rows * a.group / ROWS) + a.c.seqs;
-  return launch_kernel(kv8_portion_kernel<DP, T>, dim3((unsigned)slots * a.c.kv_heads), dim3(THREADS), S::SMEM, s, true, a, slots);
+  const int slots = (int)((int64_t)a.rows * a.group / (S::TILES * ROWS)) + a.c.seqs;
+  return launch_kernel(kv8_portion_kernel<DP, T>, dim3((unsigned)slots * a.c.kv_heads), dim3(S::THREADS), S::SMEM, s, true, a, slots);
 }
 template <int DP, typename T>
 cudaError_t allow() {
