@@ -65,6 +65,12 @@ __device__ __forceinline__ unsigned long long add_two(unsigned long long a, unsi
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// True in one lane of a converged warp; what the others compute beside it stays in uniform registers, which the products' operands need.
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <int DP, typename T>
@@ -82,7 +88,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
   uint8_t* stages = base + S::QUERIES;
   volatile int* failed = &failed_flag;
   const Kv8View& c = a.c;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(ALL_LANES, tid >> 5, 0), lane = tid & 31;
   grid_dep_launch();
   grid_dep_wait();
 
@@ -299,30 +305,33 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
     tc_fence_before();
   } else if (warp == SOFTMAX_WARPS) {
     // ---- products
-    if (lane == 0 && pieces > 0) {
+    if (pieces > 0) {
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(TOKENS >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       const uint64_t q_desc = umma_desc_sw128(base), kv_desc = umma_desc_sw128(stages);
       RingCursor ahead, now;  // the stage whose scores are next, and the one whose values are
       auto scores = [&](int j) {
-        if (!mbar_wait(&full[ahead.stage], ahead.parity, failed, nullptr, 0)) return false;
+        if (!__all_sync(ALL_LANES, mbar_wait(&full[ahead.stage], ahead.parity, failed, nullptr, 0))) return false;
         tc_fence_after();
         const uint64_t dk = kv_desc + ahead.stage * (S::STAGE >> 4);
         for (int t = 0; t < tiles; ++t) {
           const uint32_t to = o_of(t) + DP + (uint32_t)(j & 1) * 64;
           const uint64_t dq = q_desc + (uint32_t)t * (S::TILE_QUERIES >> 4);
+          if (elected()) {
 #pragma unroll
-          for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+            for (int p = 0; p < (PAIR ? 2 : 1); ++p)
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-              umma_bf16_ss(to, dq + (uint32_t)((p * KC + (k >> 2)) * (16384 >> 4) + (k & 3) * 2), dk + (uint32_t)((k >> 2) * (8192 >> 4) + (k & 3) * 2),
-                           idesc_s, (p | k) != 0);
-          umma_commit(&s_full[t][j & 1]);
+              for (int k = 0; k < DP / 16; ++k)
+                umma_bf16_ss(to, dq + (uint32_t)((p * KC + (k >> 2)) * (16384 >> 4) + (k & 3) * 2), dk + (uint32_t)((k >> 2) * (8192 >> 4) + (k & 3) * 2),
+                             idesc_s, (p | k) != 0);
+            umma_commit(&s_full[t][j & 1]);
+          }
+          __syncwarp();
         }
         ahead.next(STAGES);
         return true;
       };
-      for (int t = 0; t < tiles && ok; ++t) ok = mbar_wait(&q_full[t], 0, failed, nullptr, 0);
+      for (int t = 0; t < tiles && ok; ++t) ok = __all_sync(ALL_LANES, mbar_wait(&q_full[t], 0, failed, nullptr, 0));
       if (ok && STAGES > 1) ok = scores(0);
       for (int j = 0; j < pieces && ok; ++j) {
         if (STAGES > 1) {
@@ -332,18 +341,21 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
         }
         const uint64_t dv = kv_desc + (uint32_t)(now.stage * (S::STAGE >> 4) + (S::HALF >> 4));
         for (int t = 0; t < tiles && ok; ++t) {
-          ok = mbar_wait(&p_full[t][j & 1], (j >> 1) & 1, failed, nullptr, 0);
+          ok = __all_sync(ALL_LANES, mbar_wait(&p_full[t][j & 1], (j >> 1) & 1, failed, nullptr, 0));
           if (!ok) break;
           tc_fence_after();
           const uint32_t to = o_of(t), from = to + DP + (uint32_t)(j & 1) * 64;
+          if (elected()) {
 #pragma unroll
-          for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+            for (int p = 0; p < (PAIR ? 2 : 1); ++p)
 #pragma unroll
-            for (int k = 0; k < TOKENS / 16; ++k)
-              umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (j | p | k) != 0);
-          umma_commit(&o_done[t]);
+              for (int k = 0; k < TOKENS / 16; ++k)
+                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (j | p | k) != 0);
+            umma_commit(&o_done[t]);
+            if (t == tiles - 1) umma_commit(&empty[now.stage]);
+          }
+          __syncwarp();
         }
-        if (ok) umma_commit(&empty[now.stage]);
         now.next(STAGES);
       }
     }
