@@ -2,18 +2,22 @@
 //
 // A CTA has one or two tiles of 128 (token, query head of the group) rows that share a key / value head, and walks the pieces of 64
 // positions that any of them sees. Both products are tcgen05 instructions on FP16 operands: S = Q K^T with both in shared memory, O += P V
-// with P in tensor memory in the place of S and O in tensor memory. Four producer warps load codes (sent for one piece ahead, in
+// with P in tensor memory in the place of S and O in tensor memory. Producer warps load codes (sent for one piece ahead, in
 // registers), turn them into FP16 (exact) and store them with the operands' 128-byte swizzle: keys lie by token, values by head entry,
 // so both are K-major as they come. Four softmax warps for each tile have a row for every thread, which needs no exchange between
 // threads; one warp issues the products, the scores of a piece in front of the values of the one before it, so that the tensor pipe
-// works while the softmax of the next scores is computed. Two tiles (head_dim up to 128: tensor memory holds both) share the
-// producers' work, and one's softmax runs beside the other's products.
+// works while the softmax of the next scores is computed. Two tiles share the producers' work at head_dim 128 (1500 rows behind 2600
+// positions, 32 query heads: 233 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are better (1000
+// rows of four sequences, 12 heads: 42 us, 55 us), above 128 tensor memory has room for one.
+// Where the tiles are too few for the chip, each is cut along the positions (grid z); the parts, FP32 with their maxima and sums, are
+// merged by a kernel of their own in the order of the positions.
 //
 // Scales, weights and the running maximum are those of the step kernel: the value scale is part of the exponent, the denominator
 // divides it out. The maximum that weights refer to moves only when a row outgrows it by 2^8 (FP16 holds 2^15), which spares most
 // passes over O. FP32 rows are pairs of FP16 numbers, queries and weights alike: two products into the same accumulator.
 // Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy
 // at head_dim 128, 1024 cycles for 256 rows and 64 positions.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -22,17 +26,19 @@
 namespace pg {
 namespace {
 
-constexpr int ROWS = 128, TOKENS = 64, TILE_WARPS = 4, PRODUCER_WARPS = 4;
+constexpr int ROWS = 128, TOKENS = 64, TILE_WARPS = 4;
 
 template <int DP, typename T>
 struct PortionShape {
   static constexpr bool PAIR = std::is_same<T, float>::value;
-  static constexpr int KC = DP / 64, TILES = DP <= 128 ? 2 : 1;
+  static constexpr int KC = DP / 64, TILES = DP == 128 ? 2 : 1;
+  static constexpr int PRODUCER_WARPS = DP == 64 ? 3 : 4;  // (3: eight warps in all, which leaves two CTAs 128 registers a thread)
   static constexpr int SOFTMAX_WARPS = TILES * TILE_WARPS, THREADS = (SOFTMAX_WARPS + 1 + PRODUCER_WARPS) * 32;
   static constexpr int TILE_QUERIES = (PAIR ? 2 : 1) * KC * 16384, QUERIES = TILES * TILE_QUERIES, HALF = KC * 8192, STAGE = 2 * HALF;  // bytes
-  static constexpr int STAGES = QUERIES + 3 * STAGE <= 192 * 1024 ? 3 : QUERIES + 2 * STAGE <= 192 * 1024 ? 2 : 1;
+  static constexpr int STAGES = QUERIES + 3 * STAGE <= (DP == 64 ? 100 : 192) * 1024 ? 3 : QUERIES + 2 * STAGE <= 192 * 1024 ? 2 : 1;
   static constexpr int SMEM = QUERIES + STAGES * STAGE + 1024;
-  static constexpr int COLS = 512;  // tensor memory: for each tile O, then two places for scores and weights
+  static constexpr int CTAS = DP == 64 ? 2 : 1;  // for an SM
+  static constexpr int COLS = 512 / CTAS;  // tensor memory: for each tile O, then two places for scores and weights
   static_assert(TILES * (DP + 128) <= COLS, "tensor memory");
 };
 
@@ -73,12 +79,44 @@ __device__ __forceinline__ bool elected() {
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Rows of one CTA (slot) and the pieces of 64 positions that they see: [0, kept) and [low, high). A sequence has the slots from
+// floor(its first row * group / size) + its number on; the last rows, which see most, come first.
+struct Portion {
+  SeqRows r;
+  int b, row0, rows, len, have, pos_low, pos_high, low, kept, pieces, parts;
+  __device__ __forceinline__ Portion(const Kv8AttnArgs& a, int slot, int size, int most_parts) {
+    const Kv8View& c = a.c;
+    auto first_slot = [&](int s) { return (int)((int64_t)min(max(a.row_start[s], 0), a.rows) * a.group / size) + s; };
+    int lo = 0, hi = c.seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first_slot(mid) <= slot) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    r = seq_rows(a.row_start, a.rows, b);
+    row0 = (slot - first_slot(b)) * size;
+    rows = min(size, r.n * a.group - row0);
+    if (row0 < 0 || r.n * a.group <= a.step_rows) rows = 0;  // none, or so few that the step kernel has them
+    if (rows <= 0) return;
+    len = max(a.lens[b], 0);
+    have = min(len, c.pages_per_seq << c.page_shift);
+    pos_low = len - r.n + row0 / a.group;
+    pos_high = len - r.n + (row0 + rows - 1) / a.group;
+    const int high = (max(min(pos_high + 1, have), 0) + TOKENS - 1) / TOKENS;
+    low = a.window > 0 ? min(max(pos_low - a.window + 1, 0) / TOKENS, high) : 0;
+    kept = min((min(a.keep, have) + TOKENS - 1) / TOKENS, low);
+    pieces = kept + high - low;
+    parts = max(1, min(most_parts, pieces / 4));  // not so many that a part is all beginning and end
+  }
+};
+
 template <int DP, typename T>
-__global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_kernel(Kv8AttnArgs a, int slots) {
+__global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP, T>::CTAS) kv8_portion_kernel(Kv8AttnArgs a, int slots) {
   using S = PortionShape<DP, T>;
   constexpr bool PAIR = S::PAIR;
   constexpr int KC = S::KC, STAGES = S::STAGES, TILES = S::TILES, SOFTMAX_WARPS = S::SOFTMAX_WARPS;
-  constexpr int ITEMS = DP / 32;  // 16-byte items of keys (and of values) for every producer thread
+  constexpr int PRODUCERS = S::PRODUCER_WARPS * 32, COUNT = DP * 4, ITEMS = (COUNT + PRODUCERS - 1) / PRODUCERS;  // 16-byte items of keys (and of values): in all, for a thread
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t q_full[TILES], full[STAGES], empty[STAGES], s_full[TILES][2], p_full[TILES][2], o_done[TILES];
   __shared__ uint32_t tmem_slot;
@@ -92,30 +130,19 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
   grid_dep_launch();
   grid_dep_wait();
 
-  // ---- the tile: slots of a sequence begin at floor(first row * group / its rows) + b; the longest rows of a sequence first
   const int slot = slots - 1 - (int)(blockIdx.x / c.kv_heads), head = blockIdx.x % c.kv_heads;
-  auto first_slot = [&](int s) { return (int)((int64_t)min(max(a.row_start[s], 0), a.rows) * a.group / (TILES * ROWS)) + s; };
-  int lo = 0, hi = c.seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first_slot(mid) <= slot) lo = mid;
-    else hi = mid;
-  }
-  const int b = lo;
-  const SeqRows r = seq_rows(a.row_start, a.rows, b);
-  const int row0 = (slot - first_slot(b)) * (TILES * ROWS), rows = min(TILES * ROWS, r.n * a.group - row0);
-  if (row0 < 0 || rows <= 0 || r.n * a.group <= a.step_rows) return;  // few rows: the step kernel's
-  const int len = max(a.lens[b], 0), have = min(len, c.pages_per_seq << c.page_shift);
-  const int pos_low = len - r.n + row0 / a.group, pos_high = len - r.n + (row0 + rows - 1) / a.group;
-  const int high = (max(min(pos_high + 1, have), 0) + TOKENS - 1) / TOKENS;
-  const int low = a.window > 0 ? min(max(pos_low - a.window + 1, 0) / TOKENS, high) : 0;
-  const int kept = min((min(a.keep, have) + TOKENS - 1) / TOKENS, low), pieces = kept + high - low;
+  const Portion w(a, slot, TILES * ROWS, gridDim.y);
+  if (w.rows <= 0 || (int)blockIdx.y >= w.parts) return;
+  const int b = w.b, row0 = w.row0, rows = w.rows, len = w.len, have = w.have, pos_low = w.pos_low, pos_high = w.pos_high, low = w.low, kept = w.kept;
+  const SeqRows r = w.r;
+  // this CTA's pieces, numbered from 0
+  const int first = w.pieces * (int)blockIdx.y / w.parts, pieces = w.pieces * ((int)blockIdx.y + 1) / w.parts - first;
   const int tiles = rows > ROWS ? TILES : 1;  // that have rows
-  auto start_of = [&](int j) { return (j < kept ? j : low + j - kept) * TOKENS; };
+  auto start_of = [&](int j) { return (first + j < kept ? first + j : low + first + j - kept) * TOKENS; };
 
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], PRODUCER_WARPS);
+      mbar_init(&full[i], S::PRODUCER_WARPS);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < TILES; ++i) {
@@ -265,6 +292,9 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
         tmem_st8(s_at + (h >> 1) * 32 + (h & 1) * 8, hi16);
         if (PAIR) tmem_st8(s_at + (h >> 1) * 32 + 16 + (h & 1) * 8, lo16);
       }
+      // each product is waited for before the next one can be issued: a wait by parity knows two phases apart no more (by now it is done)
+      if (j > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (j - 1) & 1, failed, nullptr, 0));
+      if (!ok) break;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -273,8 +303,11 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
     if (ok && used && pieces > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (pieces - 1) & 1, failed, nullptr, 0));
     if (ok && used) {
       tc_fence_after();
-      const float by = sum == 0.f ? 0.f : 1.f / sum;
+      const bool part = w.parts > 1;
+      const float by = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
       T* out = (T*)a.out + (size_t)(r.first + tok) * a.out_row + (size_t)(head * a.group + g) * c.dim;
+      float* to = a.partials + (((size_t)blockIdx.x * gridDim.y + blockIdx.y) * (TILES * ROWS) + i) * (DP + 2);
+      if (part && i < rows) *reinterpret_cast<float2*>(to + DP) = make_float2(m_ref, sum);
       const bool wide_out = c.dim % 8 == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll 1
       for (int d = 0; d < c.dim; d += 16) {
@@ -285,9 +318,12 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0.f;
         }
+        if (i < rows && part) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] *= by;
-        if (i < rows) {
+          for (int e = 0; e < 16; e += 2) *reinterpret_cast<float2*>(to + d + e) = make_float2(o[e], o[e + 1]);
+        } else if (i < rows) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] *= by;
 #pragma unroll
           for (int e = 0; e < 16; e += 8) {
             if (wide_out && d + e + 8 <= c.dim) {
@@ -300,6 +336,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
             }
           }
         }
+        __syncwarp();
       }
     }
     tc_fence_before();
@@ -378,17 +415,18 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
       if (page >= 0) scale = *reinterpret_cast<const float2*>(c.scales + ((size_t)page * c.kv_heads + head) * 2);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int idx = i * 128 + p_tid, t = idx / (DP / 16), d = (idx - t * (DP / 16)) * 16;
-        const int pg_k = __shfl_sync(ALL_LANES, page, t >> 4);
+        const int idx = i * PRODUCERS + p_tid, t = idx / (DP / 16), d = (idx - t * (DP / 16)) * 16;
+        const int pg_k = __shfl_sync(ALL_LANES, page, (t >> 4) & 3);
         kr[i] = make_uint4(0, 0, 0, 0);
-        if (pg_k >= 0) kr[i] = __ldg(reinterpret_cast<const uint4*>(c.pool + ((size_t)pg_k * c.kv_heads + head) * 2 * block + (size_t)((t0 + t) & mask) * DP + d));
+        if (pg_k >= 0 && idx < COUNT)
+          kr[i] = __ldg(reinterpret_cast<const uint4*>(c.pool + ((size_t)pg_k * c.kv_heads + head) * 2 * block + (size_t)((t0 + t) & mask) * DP + d));
       }
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int d = i * 32 + (p_tid >> 2);  // piece p_tid % 4 = lane % 4: this lane's own page
+        const int idx = i * PRODUCERS + p_tid;  // head entry idx / 4; piece idx % 4 = lane % 4: this lane's own page
         vr[i] = make_uint4(0, 0, 0, 0);
-        if (page >= 0)
-          vr[i] = __ldg(reinterpret_cast<const uint4*>(c.pool + (((size_t)page * c.kv_heads + head) * 2 + 1) * block + ((size_t)d << c.page_shift) +
+        if (page >= 0 && idx < COUNT)
+          vr[i] = __ldg(reinterpret_cast<const uint4*>(c.pool + (((size_t)page * c.kv_heads + head) * 2 + 1) * block + ((size_t)(idx >> 2) << c.page_shift) +
                                                        ((t0 + (lane & 3) * 16) & mask)));
       }
     };
@@ -407,7 +445,8 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
       const int live = have - (start_of(j) + (lane & 3) * 16);  // of this lane's 16 tokens of values; bytes behind them may be anything
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int idx = i * 128 + p_tid, t = idx / (DP / 16), u = idx - t * (DP / 16);
+        const int idx = i * PRODUCERS + p_tid, t = idx / (DP / 16), u = idx - t * (DP / 16);
+        if (idx >= COUNT) continue;
         uint4 x, y;
         halves(kr[i], x, y);
         uint8_t* to = ks + (u >> 2) * 8192 + t * 128;
@@ -416,7 +455,8 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
       }
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int d = i * 32 + (p_tid >> 2);
+        const int idx = i * PRODUCERS + p_tid, d = idx >> 2;
+        if (idx >= COUNT) continue;
         if (live < 16) {
           auto keep_bytes = [&](uint32_t& w, int k) { w = live >= k + 4 ? w : live <= k ? 0u : w & ((1u << 8 * (live - k)) - 1); };
           keep_bytes(vr[i].x, 0);
@@ -451,11 +491,51 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, 1) kv8_portion_k
   if (warp == SOFTMAX_WARPS) tmem_dealloc(tmem, S::COLS);
 }
 
+// Puts the parts of a row together: a warp for a row.
+template <int DP, typename T>
+__global__ void __launch_bounds__(128) kv8_portion_merge_kernel(Kv8AttnArgs a, int slots, int most_parts) {
+  constexpr int SIZE = PortionShape<DP, T>::TILES * ROWS;
+  grid_dep_launch();
+  grid_dep_wait();
+  const Kv8View& c = a.c;
+  const int slot = slots - 1 - (int)(blockIdx.x / c.kv_heads), head = blockIdx.x % c.kv_heads;
+  const Portion w(a, slot, SIZE, most_parts);
+  const int i = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i >= w.rows || w.parts <= 1) return;
+  const float* from = a.partials + ((size_t)blockIdx.x * most_parts * SIZE + i) * (DP + 2);
+  const size_t step = (size_t)SIZE * (DP + 2);
+  // a lane for a part (at most 32): its maximum, what it is to be multiplied with
+  const float2 ml = lane < w.parts ? *reinterpret_cast<const float2*>(from + lane * step + DP) : make_float2(-INFINITY, 0.f);
+  const float top = lane_max(ml.x), f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - top), sum = lane_sum(ml.y * f);
+  const float by = sum == 0.f ? 0.f : 1.f / sum;
+  const int x = w.row0 + i, tok = x / a.group;
+  T* out = (T*)a.out + (size_t)(w.r.first + tok) * a.out_row + (size_t)(head * a.group + (x - tok * a.group)) * c.dim;
+  float o[DP / 32];
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k) o[k] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < w.parts; ++z) {
+    const float fz = __shfl_sync(ALL_LANES, f, z);
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k)
+      if (lane + 32 * k < c.dim) o[k] = fmaf(from[z * step + lane + 32 * k], fz, o[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k)
+    if (lane + 32 * k < c.dim) out[lane + 32 * k] = from_f32<T>(o[k] * by);
+}
+
 template <int DP, typename T>
 cudaError_t run(const Kv8AttnArgs& a, cudaStream_t s) {
   using S = PortionShape<DP, T>;
-  const int slots = (int)((int64_t)a.rows * a.group / (S::TILES * ROWS)) + a.c.seqs;
-  return launch_kernel(kv8_portion_kernel<DP, T>, dim3((unsigned)slots * a.c.kv_heads), dim3(S::THREADS), S::SMEM, s, true, a, slots);
+  constexpr int SIZE = S::TILES * ROWS;
+  const int slots = (int)((int64_t)a.rows * a.group / SIZE) + a.c.seqs;
+  // parts of a tile along the positions: as many as give every SM a CTA, no more than the workspace and a warp's lanes hold
+  const int64_t ctas = (int64_t)slots * a.c.kv_heads;
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(32, KV8_MAX_CTAS / ctas));
+  const cudaError_t e = launch_kernel(kv8_portion_kernel<DP, T>, dim3((unsigned)ctas, parts), dim3(S::THREADS), S::SMEM, s, true, a, slots);
+  if (e != cudaSuccess || parts == 1) return e;
+  return launch_kernel(kv8_portion_merge_kernel<DP, T>, dim3((unsigned)ctas, SIZE / 4), dim3(128), 0, s, true, a, slots, parts);
 }
 template <int DP, typename T>
 cudaError_t allow() {

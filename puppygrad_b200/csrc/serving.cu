@@ -116,7 +116,8 @@ size_t counter_bytes(const pg_kv8_cache* c, int rows, int heads) {
 }
 size_t partial_bytes(const pg_kv8_cache* c) {
   const int padded = kv8_padded(c->head_dim), rows = padded == 64 ? (2 + 16) * 16 : std::max((2 + 16) * 8, (2 + 8) * 16);
-  return (size_t)KV8_MAX_CTAS * rows * (padded + 2) * 4;
+  // (the portion kernel, which runs behind the step kernel, cuts its tiles of 128 or 256 rows into as many parts)
+  return (size_t)KV8_MAX_CTAS * std::max(rows, padded == 128 ? 256 : 128) * (padded + 2) * 4;
 }
 
 }  // namespace

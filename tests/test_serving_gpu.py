@@ -111,6 +111,12 @@ ATTENTION = [
     ([1500, 90], [700, 1], 4, 2, 80, 64, 333, 70),
     ([600], [600], 3, 1, 2, 32, 5, 0),
     ([777, 512], [500, 512], 8, 8, 64, 64, 0, 0),
+    # ... few of them, far into a sequence: cut along the positions
+    ([9000], [130], 2, 1, 128, 64, 0, 0),
+    ([5000], [70], 4, 2, 64, 32, 0, 0),
+    ([4100], [200], 1, 1, 256, 64, 0, 0),
+    ([6000, 300], [40, 35], 4, 1, 96, 16, 3000, 100),
+    ([2100], [90], 3, 1, 192, 64, 0, 0),
 ]
 
 
