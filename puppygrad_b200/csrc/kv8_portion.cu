@@ -13,7 +13,7 @@
 // merged by a kernel of their own in the order of the positions.
 //
 // Scales, weights and the running maximum are those of the step kernel: the value scale is part of the exponent, the denominator
-// divides it out. The maximum that weights refer to moves only when a row outgrows it by 2^8 (FP16 holds 2^15), which spares most
+// divides it out. The maximum (a whole number: less the blocks' exponents it is exact) that weights refer to moves only when a row outgrows it by 2^8 (FP16 holds 2^15), which spares most
 // passes over O. FP32 rows are pairs of FP16 numbers, queries and weights alike: two products into the same accumulator.
 // Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy
 // at head_dim 128, 1024 cycles for 256 rows and 64 positions.
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         t_max = fmaxf(t_max, fmaf(m, kf[h], ev[h]));
       }
       if (__any_sync(ALL_LANES, t_max > m_ref + 8.f)) {
-        const float m_new = fmaxf(m_ref, t_max), corr = m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new);
+        const float m_new = fmaxf(m_ref, ceilf(t_max)), corr = m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new);
         m_ref = m_new;
         sum *= corr;
         if (j > 0) {
@@ -356,11 +356,11 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
           const uint64_t dq = q_desc + (uint32_t)t * (S::TILE_QUERIES >> 4);
           if (elected()) {
 #pragma unroll
-            for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+            for (int p = PAIR ? 1 : 0; p >= 0; --p)  // the rests first: the sums are cut off
 #pragma unroll
               for (int k = 0; k < DP / 16; ++k)
                 umma_bf16_ss(to, dq + (uint32_t)((p * KC + (k >> 2)) * (16384 >> 4) + (k & 3) * 2), dk + (uint32_t)((k >> 2) * (8192 >> 4) + (k & 3) * 2),
-                             idesc_s, (p | k) != 0);
+                             idesc_s, p != (PAIR ? 1 : 0) || k != 0);
             umma_commit(&s_full[t][j & 1]);
           }
           __syncwarp();
@@ -384,10 +384,10 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
           const uint32_t to = o_of(t), from = to + DP + (uint32_t)(j & 1) * 64;
           if (elected()) {
 #pragma unroll
-            for (int p = 0; p < (PAIR ? 2 : 1); ++p)
+            for (int p = PAIR ? 1 : 0; p >= 0; --p)
 #pragma unroll
               for (int k = 0; k < TOKENS / 16; ++k)
-                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (j | p | k) != 0);
+                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, j != 0 || p != (PAIR ? 1 : 0) || k != 0);
             umma_commit(&o_done[t]);
             if (t == tiles - 1) umma_commit(&empty[now.stage]);
           }

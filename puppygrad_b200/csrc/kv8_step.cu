@@ -15,7 +15,7 @@
 //
 // Softmax with the blocks' scales: the key scale multiplies the score, the value scale is part of the exponent, w = 2^(s log2 e +
 // log2 scale_v - m), so that O = sum w code and the weights stay within [0, 1] however the scales differ; the denominator adds w /
-// scale_v. m is the running maximum of that exponent. FP32 queries and their weights are pairs of FP16 numbers, two instructions
+// scale_v. m is the running maximum of that exponent, rounded up. FP32 queries and their weights are pairs of FP16 numbers, two instructions
 // into one accumulator: FP32 grade. Rounding: BF16 queries are exact in FP16 after their row's scaling to [1, 2), their weights round
 // to FP16 (2^-12 of the largest).
 #include <algorithm>
@@ -330,8 +330,9 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
       m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 2));
       // exponents within +-100 keep both the factor and its inverse normal numbers
       const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 - ex) << 23);
-      const float b = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23);
+      // the sign of the score's factor goes to the queries, so that the largest product is the largest score
+      const float f = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), a.scale);
+      const float b = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23);
       back[n][0] = __shfl_sync(ALL_LANES, b, cc * 8);
       back[n][1] = __shfl_sync(ALL_LANES, b, cc * 8 + 4);
 #pragma unroll
@@ -393,14 +394,27 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
           for (int j = 0; j < 4; ++j) {  // tokens of rows r and r + 8: key rows 2 j and 2 j + 1 of the lane
             const uint4 k0 = shared16(from + 2 * j * 512), k1 = shared16(from + (2 * j + 1) * 512);
             const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+            uint32_t f[4][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t f0 = e4m3x2_to_f16x2(w0[e] & 0xFFFFu), f1 = e4m3x2_to_f16x2(w1[e] & 0xFFFFu), f2 = e4m3x2_to_f16x2(w0[e] >> 16),
-                             f3 = e4m3x2_to_f16x2(w1[e] >> 16);
+              f[e][0] = e4m3x2_to_f16x2(w0[e] & 0xFFFFu);
+              f[e][1] = e4m3x2_to_f16x2(w1[e] & 0xFFFFu);
+              f[e][2] = e4m3x2_to_f16x2(w0[e] >> 16);
+              f[e][3] = e4m3x2_to_f16x2(w1[e] >> 16);
+            }
 #pragma unroll
-              for (int n = 0; n < NB; ++n) {
-                mma_f16(s[j][n], f0, f1, f2, f3, qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
-                if constexpr (PAIR) mma_f16(s[j][n], f0, f1, f2, f3, ql[n][i * 4 + e][0], ql[n][i * 4 + e][1]);
+            for (int n = 0; n < NB; ++n) {
+              if constexpr (PAIR) {  // the rests first, and the sum in registers: the instruction cuts off what it adds
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], ql[n][i * 4 + e][0], ql[n][i * 4 + e][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][n][e] += d[e];
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_f16(s[j][n], f[e][0], f[e][1], f[e][2], f[e][3], qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
               }
             }
           }
@@ -412,51 +426,48 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
         const bool whole = __all_sync(ALL_LANES, cur.page >= 0) && t0 + UNIT - 1 <= pos_low && t0 + UNIT <= t.have &&
                            (a.window == 0 || t0 > pos_high - a.window || t0 + UNIT <= a.keep);
         uint32_t ph[NB][8], pl[PAIR ? NB : 1][8];
+        float down[NB][2];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const float f0 = back[n][0] * cur.scale.x, f1 = back[n][1] * cur.scale.x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[j][n][0] = fmaf(s[j][n][0], f0, ev);
-            s[j][n][1] = fmaf(s[j][n][1], f1, ev);
-            s[j][n][2] = fmaf(s[j][n][2], f0, ev);
-            s[j][n][3] = fmaf(s[j][n][3], f1, ev);
-          }
+          float f0 = back[n][0] * cur.scale.x, f1 = back[n][1] * cur.scale.x, add = ev;
           if (!whole) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int k = tok + 4 * j + (e & 2), p = pos[n][e & 1];
-                if (!(cur.page >= 0 && k <= p && k < t.have && (a.window == 0 || k > p - a.window || k < a.keep))) s[j][n][e] = -INFINITY;
+                const bool seen = cur.page >= 0 && k <= p && k < t.have && (a.window == 0 || k > p - a.window || k < a.keep);
+                s[j][n][e] = seen ? fmaf(s[j][n][e], e & 1 ? f1 : f0, ev) : -INFINITY;
               }
+            f0 = f1 = 1.f;
+            add = 0.f;
           }
-          // ---- running maximum and denominator
-          float top[2] = {m[n][0], m[n][1]};
+          // ---- running maximum and denominator; the maximum rounded up to a whole number, so that less the blocks' exponents it is exact
+          float raw[2] = {fmaxf(s[0][n][0], s[0][n][2]), fmaxf(s[0][n][1], s[0][n][3])};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            top[0] = fmaxf(top[0], fmaxf(s[j][n][0], s[j][n][2]));
-            top[1] = fmaxf(top[1], fmaxf(s[j][n][1], s[j][n][3]));
+          for (int j = 1; j < 4; ++j) {
+            raw[0] = fmaxf(raw[0], fmaxf(s[j][n][0], s[j][n][2]));
+            raw[1] = fmaxf(raw[1], fmaxf(s[j][n][1], s[j][n][3]));
           }
+          float top[2] = {fmaxf(m[n][0], ceilf(fmaf(raw[0], f0, add))), fmaxf(m[n][1], ceilf(fmaf(raw[1], f1, add)))};
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
             top[0] = fmaxf(top[0], __shfl_xor_sync(ALL_LANES, top[0], off));
             top[1] = fmaxf(top[1], __shfl_xor_sync(ALL_LANES, top[1], off));
           }
-          float down[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float base = top[e] == -INFINITY ? 0.f : top[e];
-            down[e] = ex2(m[n][e] - base);
+            down[n][e] = ex2(m[n][e] - base);
             m[n][e] = top[e];
-            top[e] = base;
+            top[e] = add - base;
           }
           float sum[2] = {0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              s[j][n][e] = ex2(s[j][n][e] - top[e & 1]);
+              s[j][n][e] = ex2(fmaf(s[j][n][e], e & 1 ? f1 : f0, top[e & 1]));
               sum[e & 1] += s[j][n][e];
             }
             const uint32_t h0 = pack_f16(s[j][n][0], s[j][n][1]), h1 = pack_f16(s[j][n][2], s[j][n][3]);
@@ -469,11 +480,7 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
             }
           }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) l[n][e] = fmaf(sum[e], inv_v, l[n][e] * down[e]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][n][e] *= down[e & 1];
+          for (int e = 0; e < 2; ++e) l[n][e] = fmaf(sum[e], inv_v, l[n][e] * down[n][e]);
         }
         // bytes behind the sequence's end may be anything, and 0 times NaN is NaN
         const int live = t.have - t0 - cc * 16;
@@ -490,15 +497,25 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
               keep_bytes(v1.x, 0); keep_bytes(v1.y, 4); keep_bytes(v1.z, 8); keep_bytes(v1.w, 12);
             }
             const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+            uint32_t f[4][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t f0 = e4m3x2_to_f16x2(w0[e] & 0xFFFFu), f1 = e4m3x2_to_f16x2(w1[e] & 0xFFFFu), f2 = e4m3x2_to_f16x2(w0[e] >> 16),
-                             f3 = e4m3x2_to_f16x2(w1[e] >> 16);
+              f[e][0] = e4m3x2_to_f16x2(w0[e] & 0xFFFFu);
+              f[e][1] = e4m3x2_to_f16x2(w1[e] & 0xFFFFu);
+              f[e][2] = e4m3x2_to_f16x2(w0[e] >> 16);
+              f[e][3] = e4m3x2_to_f16x2(w1[e] >> 16);
+            }
 #pragma unroll
-              for (int n = 0; n < NB; ++n) {
-                mma_f16(o[i * 4 + j][n], f0, f1, f2, f3, ph[n][2 * e], ph[n][2 * e + 1]);
-                if constexpr (PAIR) mma_f16(o[i * 4 + j][n], f0, f1, f2, f3, pl[n][2 * e], pl[n][2 * e + 1]);
+            for (int n = 0; n < NB; ++n) {  // a unit's sums start from zero and join the others in registers
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+              if constexpr (PAIR) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], pl[n][2 * e], pl[n][2 * e + 1]);
               }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], ph[n][2 * e], ph[n][2 * e + 1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[i * 4 + j][n][e] = fmaf(o[i * 4 + j][n][e], down[n][e & 1], d[e]);
             }
           }
         }

@@ -5,13 +5,13 @@
 // instructions with 16 outputs as rows and 8 tokens as columns, on codes turned into 16-bit floats in registers. Order of k within a
 // tile is free as long as both operands agree: a lane takes 16 consecutive inputs (k steps of 4), so it loads 16 bytes of weights
 // (8 of outputs r and of r + 8) and 16 inputs in a row.
-//  - BF16 inputs are exact operands; a field of 4 bits or-ed into the mantissa of 128 is 128 + code.
-//  - FP32 inputs are pairs of FP16 numbers, scaled by a power of two for every 64 inputs of a row, two products into one accumulator:
-//    FP32 grade. A field of 4 bits at the low end of an FP16 mantissa is the subnormal code * 2^-24, one place further up 16
-//    times that, which inputs scaled by 16 and by 1 make up for: one instruction for two weights.
-// Neither subtracts 8 (or 136) from every weight: the accumulators start at -8 (-136) * sum x, which one more product with a constant
-// operand gives in the accumulators' own layout, once for all the outputs of a CTA. A group's sums are FP32, times the scale
-// once per 64 inputs.
+//  - BF16 inputs are exact operands; a field of 4 bits or-ed into the mantissa of 128 is 128 + code. The accumulators start at -136 sum x
+//    instead of subtracting 136 from every weight, which one more product with a constant operand gives in their own layout, once
+//    for all the outputs of a pass.
+//  - FP32 inputs are pairs of FP16 numbers, scaled by a power of two for every 64 inputs of a row, the rests' products first, then the
+//    others' into the same accumulator, and exact weights: FP32 grade (the instruction cuts off sums, so that starting far from zero
+//    would show: 1.2e-6 where this is off by 1e-7).
+// A group's sums are FP32, times the scale once per 64 inputs.
 // A CTA has a range of the tiles of 16 outputs and goes over it in passes of up to R tiles, so that 64 inputs once loaded serve R tiles. Its
 // warps take every WARPS-th tile of 64 inputs and are added up in shared memory, in order.
 #include <cuda_bf16.h>
@@ -38,11 +38,17 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Inputs 2 i and 2 i + 1 of a word of 8 codes as 16-bit floats. FP16: code * 2^-24 for even i, code * 2^-20 for odd i.
+// Inputs 2 i and 2 i + 1 of a word of 8 codes as 16-bit floats: BF16 128 + code, FP16 the weight code - 8 itself (1024 + code, or 64 + code
+// from the field one place further up, less the rest, both exact).
 template <bool PAIR>
 __device__ __forceinline__ uint32_t weights2(uint32_t word, int i) {
-  if (PAIR) return (i < 2 ? word : word >> 8) & (i & 1 ? 0x00F000F0u : 0x000F000Fu);
-  return ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
+  if (PAIR) {
+    const uint32_t u = ((i < 2 ? word : word >> 8) & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+    const __half2 h = *reinterpret_cast<const __half2*>(&u);
+    const __half2 w = i & 1 ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hsub2(h, __float2half2_rn(1032.f));
+    return *reinterpret_cast<const uint32_t*>(&w);
+  }
+  return ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
 }
 
 // 16 inputs of one row: as they come, and as operand words (word 2 s + e: inputs 4 s + 2 e and 4 s + 2 e + 1).
@@ -93,17 +99,17 @@ struct Operand<float> {
     m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 1));
     m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 2));
     const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
-    const float s = __uint_as_float((uint32_t)(127 - e) << 23), s16 = 16.f * s;
+    const float s = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float f = i & 1 ? s : s16, a = v[2 * i] * f, b = v[2 * i + 1] * f;
+      const float a = v[2 * i] * s, b = v[2 * i + 1] * s;
       const __half2 h = __floats2half2_rn(a, b);
       const float2 q = __half22float2(h);
       const __half2 l = __floats2half2_rn(a - q.x, b - q.y);
       w[0][i] = *reinterpret_cast<const uint32_t*>(&h);
       w[1][i] = *reinterpret_cast<const uint32_t*>(&l);
     }
-    return __uint_as_float((uint32_t)(127 + e + 20) << 23);
+    return __uint_as_float((uint32_t)(127 + e) << 23);
   }
 };
 
@@ -122,33 +128,38 @@ struct Tokens {
         back[t][0] = __shfl_sync(ALL_LANES, b, c * 8);
         back[t][1] = __shfl_sync(ALL_LANES, b, c * 8 + 4);
       }
-      const uint32_t even = PAIR ? 0x80088008u : 0xC308C308u, odd = PAIR ? 0x80808080u : 0xC308C308u;  // -8 in either place; -136
-      const uint32_t f[4] = {even, even, odd, odd};
 #pragma unroll
       for (int e = 0; e < 4; ++e) base[t][e] = 0.f;
+      if constexpr (!PAIR) {
+        const uint32_t f[4] = {0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u};  // -136
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) mma16<PAIR>(base[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
+        for (int s = 0; s < 4; ++s) mma16<PAIR>(base[t], f, x[t].w[0][2 * s], x[t].w[0][2 * s + 1], base[t]);
+      }
     }
   }
   // 16 outputs: this lane's codes, the scales of outputs g and g + 8.
   __device__ __forceinline__ void add(const uint4& w, uint16_t scale_a, uint16_t scale_b, float (&acc)[NT][4]) const {
-    float d[NT][4];
+    // inputs 4 s .. 4 s + 3 of outputs g (words x, y) and g + 8 (z, w)
+    uint32_t f[4][4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      // inputs 4 s .. 4 s + 3 of outputs g (words x, y) and g + 8 (z, w)
       const uint32_t wa = s < 2 ? w.x : w.y, wb = s < 2 ? w.z : w.w;
       const int i = (s & 1) * 2;
-      const uint32_t f[4] = {weights2<PAIR>(wa, i), weights2<PAIR>(wb, i), weights2<PAIR>(wa, i + 1), weights2<PAIR>(wb, i + 1)};
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          if (s + p == 0) mma16<PAIR>(d[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
-          else mma16<PAIR>(d[t], f, x[t].w[p][2 * s], x[t].w[p][2 * s + 1], d[t]);
-        }
+      f[s][0] = weights2<PAIR>(wa, i);
+      f[s][1] = weights2<PAIR>(wb, i);
+      f[s][2] = weights2<PAIR>(wa, i + 1);
+      f[s][3] = weights2<PAIR>(wb, i + 1);
     }
+    float d[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (p == PARTS - 1 && s == 0) mma16<PAIR>(d[t], f[s], x[t].w[p][2 * s], x[t].w[p][2 * s + 1], base[t]);
+          else mma16<PAIR>(d[t], f[s], x[t].w[p][2 * s], x[t].w[p][2 * s + 1], d[t]);
+        }
     const float sa = __uint_as_float((uint32_t)scale_a << 16), sb = __uint_as_float((uint32_t)scale_b << 16);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
