@@ -171,7 +171,9 @@ class _Library:
     def __getattr__(self, name):
         if _Library._lib is None:
             _Library._lib = _load()
-        return getattr(_Library._lib, name)
+        function = getattr(_Library._lib, name)
+        setattr(self, name, function)  # found without this method from now on
+        return function
 
 
 lib = _Library()

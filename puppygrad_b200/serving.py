@@ -44,6 +44,8 @@ def _device(t, name: str) -> int:
 
 def _flat(t, name: str, dtype: str, shape: Tuple[int, ...], device: int) -> int:
     """Address of a buffer that has to be contiguous and of that type and shape."""
+    if t.shape == shape and _seen.get(t.dtype) == dtype and t.is_contiguous() and t.get_device() == device:
+        return t.data_ptr()
     if t.shape != shape or _name(t.dtype) != dtype or not t.is_contiguous():
         raise _bad(f"{name}: {dtype} {shape} without gaps is needed, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
     if t.get_device() != device:
@@ -51,21 +53,21 @@ def _flat(t, name: str, dtype: str, shape: Tuple[int, ...], device: int) -> int:
     return t.data_ptr()
 
 
-def _rows(t, name: str, dtype, inner: Tuple[int, ...], device: int, rows: int) -> Tuple[int, int]:
-    """Address and distance between rows of [rows, *inner], whose rows are without gaps."""
-    if t.shape != (rows, *inner) or t.dtype != dtype:
-        raise _bad(f"{name}: {dtype} {(rows, *inner)} is needed, got {t.dtype} {tuple(t.shape)}")
+def _rows(t, name: str, dtype, shape: Tuple[int, ...], device: int) -> Tuple[int, int]:
+    """Address and distance between rows of a buffer of that type and shape, whose rows are without gaps."""
+    if t.shape != shape or t.dtype != dtype:
+        raise _bad(f"{name}: {dtype} {shape} is needed, got {t.dtype} {tuple(t.shape)}")
     if t.get_device() != device:
         raise _bad(f"{name} is on {t.device}, the others are on cuda:{device}")
-    stride, width = t.stride(), inner[-1]
-    gap = width > 1 and stride[-1] != 1
-    if len(inner) == 2:
-        gap = gap or (inner[0] > 1 and stride[1] != width)
-        width *= inner[0]
+    stride, width = t.stride(), shape[-1]
+    gap = stride[-1] != 1 and width > 1
+    if len(shape) == 3:
+        gap = gap or (stride[1] != width and shape[1] > 1)
+        width *= shape[1]
     if gap:
         raise _bad(f"{name}: a row must be without gaps, got strides {stride}")
     # of a single row (or none) the distance says nothing
-    return t.data_ptr(), stride[0] if rows > 1 else width
+    return t.data_ptr(), stride[0] if shape[0] > 1 else width
 
 
 class Kv8Cache:
@@ -95,27 +97,27 @@ class Kv8Cache:
             raise _bad(N.lib.pg_last_error_message().decode())
         return n_pages, kv_heads, size // (n_pages * kv_heads)
 
-    def _row_map(self, lens, row_start) -> Tuple[int, int]:
-        return (_flat(lens, "lens", "torch.int32", (self.seqs,), self.device),
-                0 if row_start is None else _flat(row_start, "row_start", "torch.int32", (self.seqs + 1,), self.device))
-
     def append(self, k, v, lens, row_start=None, q=None, q_out=None, rot_dims: int = 0, rot_base: float = 10000.0, stream: int = 0) -> None:
         """Appends k and v [rows, kv_heads, head_dim], k turned by its positions; q [rows, heads, head_dim] is turned into q_out (which
         may be q). Sequence b has rows row_start[b] : row_start[b + 1] (None: row b), at the last positions of lens[b], its
         length with them."""
-        rows, inner, device = k.shape[0], (self.kv_heads, self.head_dim), self.device
-        dtype = _code(k, "k")
-        kp, ks = _rows(k, "k", k.dtype, inner, device, rows)
-        vp, vs = _rows(v, "v", k.dtype, inner, device, rows)
+        rows, device, kind = k.shape[0], self.device, k.dtype
+        dtype, shape = _code(k, "k"), (rows, self.kv_heads, self.head_dim)
+        kp, ks = _rows(k, "k", kind, shape, device)
+        vp, vs = _rows(v, "v", kind, shape, device)
         qp = qs = op = os = heads = 0
         if q is not None or q_out is not None:
             if q is None or q_out is None:
                 raise _bad("q and q_out must be given together")
             heads = q.shape[1]
-            qp, qs = _rows(q, "q", k.dtype, (heads, self.head_dim), device, rows)
-            op, os = _rows(q_out, "q_out", k.dtype, (heads, self.head_dim), device, rows)
-        lp, sp = self._row_map(lens, row_start)
-        check(N.lib.pg_kv8_append(self._ref, kp, ks, vp, vs, qp, qs, op, os, dtype, heads, rows, sp, lp, rot_dims, rot_base, stream))
+            shape = (rows, heads, self.head_dim)
+            qp, qs = _rows(q, "q", kind, shape, device)
+            op, os = _rows(q_out, "q_out", kind, shape, device)
+        lp = _flat(lens, "lens", "torch.int32", (self.seqs,), device)
+        sp = 0 if row_start is None else _flat(row_start, "row_start", "torch.int32", (self.seqs + 1,), device)
+        status = N.lib.pg_kv8_append(self._ref, kp, ks, vp, vs, qp, qs, op, os, dtype, heads, rows, sp, lp, rot_dims, rot_base, stream)
+        if status:
+            check(status)
 
     def workspace_bytes(self, rows: int, heads: int, dtype) -> int:
         """Size of the workspace of `attention` calls of up to that many rows; its memory must be zero before its first use."""
@@ -130,14 +132,19 @@ class Kv8Cache:
         """out = softmax(scale * q . k) v over what each row sees; q and out [rows, heads, head_dim], scale head_dim ** -0.5 unless
         given, `lens` and `row_start` as in `append`. max_rows: at least the rows of any sequence. `workspace`: uint8, zeroed
         before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each."""
-        rows, heads = q.shape[0], q.shape[1]
-        dtype, inner = _code(q, "q"), (heads, self.head_dim)
-        qp, qs = _rows(q, "q", q.dtype, inner, self.device, rows)
-        op, os = _rows(out, "out", q.dtype, inner, self.device, rows)
-        lp, sp = self._row_map(lens, row_start)
-        wp = _flat(workspace, "workspace", "torch.uint8", (workspace.shape[0],), self.device)
-        check(N.lib.pg_kv8_attention(self._ref, qp, qs, op, os, dtype, heads, rows, max_rows, sp, lp,
-                                     self.head_dim ** -0.5 if scale is None else scale, window, keep_first, wp, workspace.shape[0], stream))
+        device, kind, shape = self.device, q.dtype, (*q.shape[:2], self.head_dim)
+        rows, heads = shape[:2]
+        dtype = _code(q, "q")
+        qp, qs = _rows(q, "q", kind, shape, device)
+        op, os = _rows(out, "out", kind, shape, device)
+        lp = _flat(lens, "lens", "torch.int32", (self.seqs,), device)
+        sp = 0 if row_start is None else _flat(row_start, "row_start", "torch.int32", (self.seqs + 1,), device)
+        size = workspace.shape[0]
+        wp = _flat(workspace, "workspace", "torch.uint8", (size,), device)
+        status = N.lib.pg_kv8_attention(self._ref, qp, qs, op, os, dtype, heads, rows, max_rows, sp, lp,
+                                        self.head_dim ** -0.5 if scale is None else scale, window, keep_first, wp, size, stream)
+        if status:
+            check(status)
 
 
 def q4_shapes(n: int, k: int, group: int) -> Tuple[Tuple[int, int, int], Tuple[int, int]]:
@@ -151,7 +158,7 @@ def quantize_q4(w, packed, scales, group: int, stream: int = 0) -> None:
     """Lays the matrix w [n, k] out in 4 bits, with one scale for every `group` (64 or 128) inputs of an output."""
     n, k = w.shape
     dtype, device = _code(w, "w"), _device(w, "w")
-    wp, ws = _rows(w, "w", w.dtype, (k,), device, n)
+    wp, ws = _rows(w, "w", w.dtype, (n, k), device)
     ps, ss = q4_shapes(n, k, group)
     check(N.lib.pg_quantize_q4(wp, ws, dtype, n, k, group, _flat(packed, "packed", "torch.uint8", ps, device),
                                _flat(scales, "scales", "torch.bfloat16", ss, device), device, stream))
@@ -160,27 +167,35 @@ def quantize_q4(w, packed, scales, group: int, stream: int = 0) -> None:
 def linear_q4(x, packed, scales, out, group: int, bias=None, stream: int = 0) -> None:
     """out [m, n] = x [m, k] @ dequant(w [n, k]).T + bias for up to 16 rows."""
     m, k = x.shape
-    n = out.shape[1]
+    n, kind = out.shape[1], x.dtype
     dtype, device = _code(x, "x"), _device(x, "x")
-    xp, xs = _rows(x, "x", x.dtype, (k,), device, m)
-    op, os = _rows(out, "out", x.dtype, (n,), device, m)
-    ps, ss = (-(-n // 16), -(-k // 64), 512), (-(-k // group) if group > 0 else 0, -(-n // 16) * 16)
-    bp = 0 if bias is None else _flat(bias, "bias", _name(x.dtype), (n,), device)
-    check(N.lib.pg_linear_q4(xp, xs, _flat(packed, "packed", "torch.uint8", ps, device), _flat(scales, "scales", "torch.bfloat16", ss, device), bp,
-                             dtype, m, n, k, group, op, os, device, stream))
+    xp, xs = _rows(x, "x", kind, (m, k), device)
+    op, os = _rows(out, "out", kind, (m, n), device)
+    tiles = -(-n // 16)
+    pp = _flat(packed, "packed", "torch.uint8", (tiles, -(-k // 64), 512), device)
+    sp = _flat(scales, "scales", "torch.bfloat16", (-(-k // group) if group > 0 else 0, tiles * 16), device)
+    bp = 0 if bias is None else _flat(bias, "bias", _name(kind), (n,), device)
+    status = N.lib.pg_linear_q4(xp, xs, pp, sp, bp, dtype, m, n, k, group, op, os, device, stream)
+    if status:
+        check(status)
 
 
 def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=None, top_logprobs=None, stream: int = 0) -> None:
     """Scores of the rows of logits [rows, vocab]: logprobs [rows] of `targets` [rows], entropy [rows], the most likely ids and their
     log probabilities [rows, k] (k up to 32), each where its output is given."""
     rows, vocab = logits.shape
-    dtype, device = _code(logits, "logits"), _device(logits, "logits")
-    lp, ls = _rows(logits, "logits", logits.dtype, (vocab,), device, rows)
+    dtype, device, each = _code(logits, "logits"), _device(logits, "logits"), (rows,)
+    lp, ls = _rows(logits, "logits", logits.dtype, (rows, vocab), device)
     if (top_ids is None) != (top_logprobs is None):
         raise _bad("top_ids and top_logprobs must be given together")
-    k = 0 if top_ids is None else top_ids.shape[1]
-    f = lambda t, name, kind, shape: 0 if t is None else _flat(t, name, kind, shape, device)
-    each = (rows,)
-    check(N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, f(targets, "targets", "torch.int32", each), f(logprobs, "logprobs", "torch.float32", each),
-                                  f(entropy, "entropy", "torch.float32", each), k, f(top_ids, "top_ids", "torch.int32", (rows, k)),
-                                  f(top_logprobs, "top_logprobs", "torch.float32", (rows, k)), device, stream))
+    tp = 0 if targets is None else _flat(targets, "targets", "torch.int32", each, device)
+    op = 0 if logprobs is None else _flat(logprobs, "logprobs", "torch.float32", each, device)
+    ep = 0 if entropy is None else _flat(entropy, "entropy", "torch.float32", each, device)
+    k = ip = vp = 0
+    if top_ids is not None:
+        k = top_ids.shape[1]
+        ip = _flat(top_ids, "top_ids", "torch.int32", (rows, k), device)
+        vp = _flat(top_logprobs, "top_logprobs", "torch.float32", (rows, k), device)
+    status = N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, tp, op, ep, k, ip, vp, device, stream)
+    if status:
+        check(status)
