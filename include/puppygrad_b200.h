@@ -369,7 +369,7 @@ uint64_t pg_kv8_pool_bytes(int32_t n_pages, int32_t page_tokens, int32_t kv_head
 
 /* Appends the keys and values of `rows` new tokens, keys rotated by their positions on the way; queries of the same rows are
  * rotated too where given. Sequence b has rows row_start[b]..row_start[b+1]-1 (row_start NULL: row b is sequence b's, rows =
- * seqs) at the last positions of lens[b], its length WITH them. k, v: [rows][kv_heads][head_dim], q and q_out: [rows][heads]
+ * seqs; it must not decrease) at the last positions of lens[b], its length WITH them. k, v: [rows][kv_heads][head_dim], q and q_out: [rows][heads]
  * [head_dim], FP32 or BF16, each with its own distance between rows; q_out may be q. rot_dims (even, 0 = none): entry i of a head
  * turns with entry i + rot_dims / 2 by position * rot_base^(-2i / rot_dims).
  * The scale of a block (a page's keys or values of one head) is the smallest power of two (from 2^-100 up) that keeps its
@@ -385,7 +385,7 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
  * window > 0 only the last `window` of them (its own included) and the first keep_first of the sequence. Rows belong to sequences
  * as in pg_kv8_append, whose `lens` it takes; query head h reads key / value head h / (heads / kv_heads). A row that sees nothing
  * gets zeros; rows outside row_start[0]..row_start[seqs]-1 are left as they were. max_rows: at least the rows of any sequence
- * (it chooses the kernels; a sequence with more is still computed). FP32 queries are computed to FP32 grade from pairs of
+ * (it chooses the kernels; a sequence with more is still computed). Where row_start decreases, rows are left out or computed twice. FP32 queries are computed to FP32 grade from pairs of
  * FP16 numbers, BF16 queries with FP16 probabilities; sums are FP32.
  * workspace: pg_kv8_attention_workspace_bytes() bytes, 256-byte aligned, zeroed by the caller before its first use and left ready for the next
  * call. Calls that may overlap on the GPU (captured graphs among them) need workspaces of their own. */
@@ -404,7 +404,7 @@ uint64_t pg_q4_scale_bytes(int32_t n, int32_t k, int32_t group);
 int pg_quantize_q4(const void* w, int64_t w_row, int32_t dtype, int32_t n, int32_t k, int32_t group, void* packed, void* scales,
                    int32_t device, void* stream);
 /* out[m][n] = x[m][k] . dequant(w)[n][k]^T + bias; 1 <= m <= 16; x, bias (may be NULL) and out FP32 or BF16. FP32 inputs are
- * computed to FP32 grade from pairs of FP16 numbers. */
+ * computed to FP32 grade from pairs of FP16 numbers. A row with a NaN, an infinity, or (BF16) a sum of 64 magnitudes above 2^120 gives NaN. */
 int pg_linear_q4(const void* x, int64_t x_row, const void* packed, const void* scales, const void* bias, int32_t dtype, int32_t m,
                  int32_t n, int32_t k, int32_t group, void* out, int64_t out_row, int32_t device, void* stream);
 

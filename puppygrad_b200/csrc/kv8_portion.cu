@@ -9,12 +9,12 @@
 // works while the softmax of the next scores is computed. Two tiles share the producers' work at head_dim 128 (1500 rows behind 2600
 // positions, 32 query heads: 233 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are better (1000
 // rows of four sequences, 12 heads: 42 us, 55 us), above 128 tensor memory has room for one.
-// Where the tiles are too few for the chip, each is cut along the positions (grid z); the parts, FP32 with their maxima and sums, are
+// Where the tiles are too few for the chip, each is cut along the positions (grid y); the parts, FP32 with their maxima and sums, are
 // merged by a kernel of their own in the order of the positions.
 //
 // Scales, weights and the running maximum are those of the step kernel: the value scale is part of the exponent, the denominator
-// divides it out. The maximum (a whole number: less the blocks' exponents it is exact) that weights refer to moves only when a row outgrows it by 2^8 (FP16 holds 2^15), which spares most
-// passes over O. FP32 rows are pairs of FP16 numbers, queries and weights alike: two products into the same accumulator.
+// divides it out. The maximum that weights refer to (a whole number: less the blocks' exponents it is exact) moves only when a row
+// outgrows it by 2^8 (FP16 holds 2^15), which spares most passes over O. FP32 rows are pairs of FP16 numbers, queries and weights alike: two products into the same accumulator.
 // Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy
 // at head_dim 128, 1024 cycles for 256 rows and 64 positions.
 #include <algorithm>
@@ -301,9 +301,10 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
       if (lane == 0) mbar_arrive(&p_full[tile][j & 1]);  // (two in turn: the next one's may come before this one is waited for)
     }
     if (ok && used && pieces > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (pieces - 1) & 1, failed, nullptr, 0));
-    if (ok && used) {
+    if (used) {
       tc_fence_after();
       const bool part = w.parts > 1;
+      if (!ok) sum = __uint_as_float(0x7FC00000u);  // a wait ran out: no result, and one that shows
       const float by = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
       T* out = (T*)a.out + (size_t)(r.first + tok) * a.out_row + (size_t)(head * a.group + g) * c.dim;
       float* to = a.partials + (((size_t)blockIdx.x * gridDim.y + blockIdx.y) * (TILES * ROWS) + i) * (DP + 2);
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
 #pragma unroll 1
       for (int d = 0; d < c.dim; d += 16) {
         float o[16];
-        if (pieces > 0) {
+        if (pieces > 0 && ok) {
           tmem_ld16(tmem_o + d, o);
         } else {
 #pragma unroll
@@ -419,15 +420,15 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         const int pg_k = __shfl_sync(ALL_LANES, page, (t >> 4) & 3);
         kr[i] = make_uint4(0, 0, 0, 0);
         if (pg_k >= 0 && idx < COUNT)
-          kr[i] = __ldg(reinterpret_cast<const uint4*>(c.pool + ((size_t)pg_k * c.kv_heads + head) * 2 * block + (size_t)((t0 + t) & mask) * DP + d));
+          kr[i] = *reinterpret_cast<const uint4*>(c.pool + ((size_t)pg_k * c.kv_heads + head) * 2 * block + (size_t)((t0 + t) & mask) * DP + d);
       }
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         const int idx = i * PRODUCERS + p_tid;  // head entry idx / 4; piece idx % 4 = lane % 4: this lane's own page
         vr[i] = make_uint4(0, 0, 0, 0);
         if (page >= 0 && idx < COUNT)
-          vr[i] = __ldg(reinterpret_cast<const uint4*>(c.pool + (((size_t)page * c.kv_heads + head) * 2 + 1) * block + ((size_t)(idx >> 2) << c.page_shift) +
-                                                       ((t0 + (lane & 3) * 16) & mask)));
+          vr[i] = *reinterpret_cast<const uint4*>(c.pool + (((size_t)page * c.kv_heads + head) * 2 + 1) * block + ((size_t)(idx >> 2) << c.page_shift) +
+                                                 ((t0 + (lane & 3) * 16) & mask));
       }
     };
     auto halves = [](const uint4& v, uint4& x, uint4& y) {

@@ -69,9 +69,10 @@ struct Span {
 };
 __device__ __forceinline__ Span span_of(const Kv8AttnArgs& a, int len, int n) {
   Span s;
-  s.high = (min(len, a.c.pages_per_seq << a.c.page_shift) + UNIT - 1) / UNIT;
+  const int have = min(len, a.c.pages_per_seq << a.c.page_shift);
+  s.high = (have + UNIT - 1) / UNIT;
   s.low = a.window > 0 ? min(max(len - n - a.window + 1, 0) / UNIT, s.high) : 0;
-  s.keep = min((min(a.keep, len) + UNIT - 1) / UNIT, s.low);
+  s.keep = min((min(a.keep, have) + UNIT - 1) / UNIT, s.low);
   if (s.units() <= 0) s.high = s.low + 1;  // rows that see nothing still get their zeros
   return s;
 }
@@ -178,8 +179,12 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
   const int per = c.seqs <= THREADS ? 1 : (c.seqs + THREADS - 1) / THREADS;
   {
     int sum = 0;
+    bool disorder = false;
 #pragma unroll 1
-    for (int b = tid * per; b < min(tid * per + per, c.seqs); ++b) sum += units_of(b);
+    for (int b = tid * per; b < min(tid * per + per, c.seqs); ++b) {
+      sum += units_of(b);
+      disorder |= a.row_start && a.row_start[b + 1] < a.row_start[b];
+    }
     int up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -189,7 +194,8 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
     if (lane == 31) wsum[warp] = up;
     scan[tid] = up;
     if (tid < WARPS * 2) part_tile[tid] = -1;
-    __syncthreads();
+    // rows of two sequences at once would make more units than can be numbered
+    if (__syncthreads_or(disorder)) return;
   }
   int total = lane < WARPS ? wsum[lane] : 0;  // lane i: units up to those of warp i's threads
 #pragma unroll

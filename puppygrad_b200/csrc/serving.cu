@@ -1,5 +1,5 @@
-// Entry points of the serving operators: checks of what the host can see, then the launch. The kernels are in kv8.cu,
-// linear_q4.cu and token_logprobs.cu.
+// Entry points of the serving operators: checks of what the host can see, then the launch. The kernels are in kv8_append.cu,
+// kv8_step.cu, kv8_portion.cu, linear_q4.cu and token_logprobs.cu.
 #include "serving.h"
 
 #include <algorithm>
@@ -184,13 +184,14 @@ int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, vo
   if (!workspace || workspace_bytes < need)
     return bad("workspace of " + std::to_string(workspace ? workspace_bytes : 0) + " bytes, " + std::to_string(need) + " needed");
   if (!aligned(workspace, 256)) return bad("workspace is not 256-byte aligned");
-  // pieces of 64 tokens of all tiles of rows are numbered with 31 bits
+  // rows of a key / value head, and pieces of 64 tokens of all tiles of rows, are numbered with 31 bits
   const int group = heads / cache->kv_heads;
   const int64_t tiles = ((int64_t)rows * group / 8 + cache->seqs) * cache->kv_heads;
-  if (tiles * (((int64_t)cache->pages_per_seq * cache->page_tokens + 63) / 64) > INT32_MAX)
+  if ((int64_t)rows * group > INT32_MAX / 2 || tiles * (((int64_t)cache->pages_per_seq * cache->page_tokens + 63) / 64) > INT32_MAX)
     return bad("rows " + std::to_string(rows) + " with tables of " + std::to_string(cache->pages_per_seq) + " pages are too many for one call");
   DeviceScope scope(cache->device);
   if (scope.rc()) return scope.rc();
+  if (window > INT32_MAX / 2) window = 0;  // wider than any table: its arithmetic stays within 32 bits
   // rows that fill less than half a tile of the portion kernel, and all of them where it has no table of rows
   const bool portions = row_start && (int64_t)group * max_rows > KV8_STEP_ROWS;
   Kv8AttnArgs a{view(cache), q, out, q_row, out_row, heads, group, rows, max_rows, row_start, lens, scale, window, window > 0 ? keep_first : 0,

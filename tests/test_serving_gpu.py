@@ -229,6 +229,70 @@ def test_attention_queries_far_from_one(size):
     check_attention(cache, q, out, [1], 0.125)
 
 
+@pytest.mark.parametrize("window,keep", [(2 ** 31 - 1, 0), (2 ** 30, 2 ** 31 - 1), (50, 40), (50, 2 ** 31 - 1), (2 ** 30 - 1, 7)])
+@pytest.mark.parametrize("rows", [[1, 3, 2], [90, 3, 70]])
+def test_attention_lengths_and_windows_at_the_end_of_32_bits(rows, window, keep):
+    """A length beyond the table stands for tokens that are not stored: its rows see those of the table that are in reach."""
+    known = [192, 64, 128]
+    cache = Cache(known, 2, 64, 64, 31, per_seq=3)
+    lens = [2 ** 31 - 1, 64, 2 ** 31 - 1]
+    n = sum(rows)
+    q = torch.randn(n, 4, 64, generator=gen(4), device=DEV)
+    out = torch.full_like(q, 7.0)
+    cache.handle.attention(q, out, i32(lens), workspace(cache, n, 4, F32), row_start=starts(rows), max_rows=max(rows), window=window, keep_first=keep)
+    at = 0
+    for b, r in enumerate(rows):
+        keys, values = cache.kv(b)
+        # (a window of 2^30 or more, wider than any table, is none)
+        want = ref.attention(q[at:at + r].double(), keys, values, torch.arange(lens[b] - r, lens[b], device=DEV), 0.125, window if window < 2 ** 30 else 0, keep)
+        assert ((out[at:at + r].double() - want).abs() <= 2.0 ** -15 * values.abs().max() + 2.0 ** -24 * want.abs()).all(), b
+        at += r
+
+
+def test_attention_row_starts_that_decrease_are_without_effect_on_later_calls():
+    cache = Cache([50, 60, 40], 1, 64, 16, 2)
+    q = torch.randn(9, 2, 64, generator=gen(1), device=DEV)
+    out, ws = torch.full_like(q, 5.0), workspace(cache, 9, 2, F32)
+    cache.handle.attention(q, out, i32([50, 60, 40]), ws, row_start=i32([0, 9, 2, 9]), max_rows=9)
+    assert (out == 5).all() and not ws[:256].any()
+    cache.handle.attention(q, out, i32([50, 60, 40]), ws, row_start=i32([0, 3, 5, 9]), max_rows=4)
+    check_attention(cache, q, out, [3, 2, 4], 0.125)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_more_sequences_than_threads_with_rows_of_all_numbers(dtype):
+    rows = [(0, 1, 1, 2, 5, 1, 33, 0, 70)[i % 9] for i in range(1100)]
+    lens = [(i * 29) % 120 for i in range(1100)]
+    cache = Cache(lens, 1, 64, 32, 13)
+    n = sum(rows)
+    q = torch.randn(n, 2, 64, generator=gen(6), device=DEV).to(dtype)
+    out = torch.full_like(q, 5.0)
+    cache.handle.attention(q, out, i32(lens), workspace(cache, n, 2, dtype), row_start=starts(rows), max_rows=70)
+    check_attention(cache, q, out, rows, 0.125)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_cache_of_more_than_4_gb(dtype):
+    """The last pages of a pool whose offsets need 33 bits: append, then both attention kernels."""
+    page, kvh, dim = 64, 8, 128
+    n_pages = (1 << 32) // (kvh * 2 * page * dim) + 40
+    pool = torch.empty(pg.Kv8Cache.pool_shape(n_pages, kvh, page, dim), dtype=torch.uint8, device=DEV)
+    assert pool.numel() > 1 << 32
+    cache = Cache([0, 0], kvh, dim, page, 3)
+    cache.pool, cache.scales = pool, torch.empty(n_pages, kvh, 2, device=DEV)
+    cache.table = torch.arange(n_pages - 8, n_pages, dtype=torch.int32, device=DEV).view(2, 4)
+    cache.handle, cache.lens = pg.Kv8Cache(pool, cache.scales, cache.table, page_tokens=page, head_dim=dim), [200, 150]
+    x = torch.randn(350, kvh, dim, generator=gen(2), device=DEV).to(dtype)
+    cache.handle.append(x, x, i32([200, 150]), row_start=starts([200, 150]))
+    keys, values = cache.kv(1)
+    assert ((values - x[200:].double()).abs() <= 0.07 * x[200:].abs().double() + 1e-2).all() and torch.equal(keys, values)
+    for rows in ([1, 1], [200, 90]):
+        q = torch.randn(sum(rows), kvh, dim, generator=gen(5), device=DEV).to(dtype)
+        out, ws = torch.empty_like(q), workspace(cache, sum(rows), kvh, dtype)
+        cache.handle.attention(q, out, i32([200, 150]), ws, row_start=starts(rows), max_rows=max(rows))
+        check_attention(cache, q, out, rows, dim ** -0.5)
+
+
 # ------------------------------------------------------------------ append
 def quantised(x, scale):
     """Half a step around each value: how far a code times its scale may be from x (both float64)."""
@@ -540,6 +604,52 @@ def test_token_logprobs_each_output_alone():
     assert torch.equal(ids.long(), want[2])
 
 
+def test_token_logprobs_rows_further_apart_than_31_bits():
+    far = (1 << 31) + 24
+    store = torch.empty(far + 5000, dtype=BF16, device=DEV)
+    x = torch.as_strided(store, (2, 5000), (far, 1))
+    x.copy_(torch.randn(2, 5000, generator=gen(3), device=DEV))
+    t, want = i32([4999, 17]), None
+    lp, ent, ids, values = torch.empty(2, device=DEV), torch.empty(2, device=DEV), torch.empty(2, 6, dtype=torch.int32, device=DEV), torch.empty(2, 6, device=DEV)
+    pg.token_logprobs(x, targets=t, logprobs=lp, entropy=ent, top_ids=ids, top_logprobs=values)
+    want = scores(x, t, 6)
+    assert ((lp - want[0]).abs() <= 2.0 ** -18 * (1 + want[0].abs())).all() and ((ent - want[1]).abs() <= 2.0 ** -18 * (1 + want[1].abs())).all()
+    assert torch.equal(ids.long(), want[2])
+
+
+def test_linear_q4_codes_beyond_32_bits():
+    n, k = 1 << 17, (1 << 16) + 64
+    ps, ss = pg.q4_shapes(n, k, 128)
+    packed, scales = torch.zeros(ps, dtype=torch.uint8, device=DEV), torch.zeros(ss, dtype=BF16, device=DEV)
+    assert packed.numel() > 1 << 32
+    packed[-1] = torch.randint(0, 256, packed[-1].shape, generator=gen(2), device=DEV).to(torch.uint8)
+    scales[:, -16:] = 0.25
+    x, out = torch.randn(3, k, generator=gen(3), device=DEV), torch.full((3, n), 5.0, device=DEV)
+    pg.linear_q4(x, packed, scales, out, 128)
+    w = ref.q4_weights(packed[-1:].clone(), scales[:, -16:].clone(), 16, k, 128)
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    tile = x.double().abs().amax(-1, keepdim=True) * w.abs().sum(-1)
+    # (a warp adds 129 sums up, half a step of 2^-24 each: within 2^-16)
+    assert ((out[:, -16:].double() - want).abs() <= 2.0 ** -16 * size + 2.0 ** -24 * want.abs() + 2.0 ** -21 * tile).all()
+    assert (out[:, :-16] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_q4_rows_that_are_not_finite_stay_alone(dtype):
+    n, k = 40, 200
+    ps, ss = pg.q4_shapes(n, k, 64)
+    packed, scales = torch.empty(ps, dtype=torch.uint8, device=DEV), torch.empty(ss, dtype=BF16, device=DEV)
+    pg.quantize_q4(torch.randn(n, k, generator=gen(1), device=DEV), packed, scales, 64)
+    x = torch.randn(12, k, generator=gen(2), device=DEV).to(dtype)
+    want, got = torch.empty(12, n, dtype=dtype, device=DEV), torch.empty(12, n, dtype=dtype, device=DEV)
+    pg.linear_q4(x, packed, scales, want, 64)
+    x[3, 7], x[9, 150], x[10, 199] = math.nan, math.inf, -math.inf
+    pg.linear_q4(x, packed, scales, got, 64)
+    odd = torch.tensor([3, 9, 10], device=DEV)
+    keep = torch.tensor([i for i in range(12) if i not in (3, 9, 10)], device=DEV)
+    assert torch.isnan(got[odd]).all() and torch.equal(got[keep], want[keep])
+
+
 # ------------------------------------------------------------------ together
 class Layer:
     """One layer's step as a serving program builds it from the operators: products in 4 bits around the 8-bit cache, then a head."""
@@ -640,3 +750,72 @@ def test_two_streams_at_once():
             c.handle.attention(q, o, l, w, stream=s.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(alone, both))
+
+
+class Prompts:
+    """Portions of prompts as a serving program has them: append, then attention, over one cache."""
+
+    def __init__(self, dtype, seed, seqs=3, heads=4, kvh=2, dim=64, room=200):
+        self.cache = empty_cache(seqs, 20, kvh, dim, 16)
+        e = lambda *s, t=dtype: torch.zeros(*s, dtype=t, device=DEV)
+        self.q, self.k, self.v, self.turned, self.out = e(room, heads, dim), e(room, kvh, dim), e(room, kvh, dim), e(room, heads, dim), e(room, heads, dim)
+        self.lens, self.start, self.g = e(seqs, t=torch.int32), e(seqs + 1, t=torch.int32), gen(seed)
+        self.ws = torch.zeros(self.cache.workspace_bytes(room, heads, dtype), dtype=torch.uint8, device=DEV)
+        for t in (self.q, self.k, self.v):
+            t.copy_(torch.randn(t.shape, generator=self.g, device=DEV))
+
+    def call(self):
+        s = torch.cuda.current_stream().cuda_stream
+        self.cache.append(self.k, self.v, self.lens, row_start=self.start, q=self.q, q_out=self.turned, rot_dims=64, stream=s)
+        self.cache.attention(self.turned, self.out, self.lens, self.ws, row_start=self.start, max_rows=200, stream=s)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_portions_of_prompts_eager_and_captured(dtype):
+    eager, captured = Prompts(dtype, 1), Prompts(dtype, 1)
+    captured.cache.page_table.copy_(eager.cache.page_table)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        captured.call()
+    lens = torch.zeros(3, dtype=torch.int32, device=DEV)
+    for rows in ([100, 40, 60], [1, 1, 1], [0, 120, 2], [50, 0, 0], [0, 0, 0], [100, 60, 40]):
+        lens += i32(rows)
+        for p in (eager, captured):
+            p.lens.copy_(lens)
+            p.start.copy_(starts(rows))
+            p.out.fill_(3.0)
+        eager.call()
+        graph.replay()
+        torch.cuda.synchronize()
+        n = sum(rows)
+        assert torch.equal(eager.out, captured.out) and (eager.out[n:] == 3).all()
+        at = 0
+        for b, r in enumerate(rows):
+            length = int(lens[b])
+            keys, values = ref.sequence_kv(eager.cache.pool, eager.cache.scales, eager.cache.page_table[b], length, 16, 64)
+            want = ref.attention(eager.turned[at:at + r].double(), keys, values, torch.arange(length - r, length, device=DEV), 0.125)
+            tol = (values.abs().max() if length else 0.0) * (2.0 ** -15 if dtype == F32 else 2.0 ** -10) + U[dtype] * want.abs()
+            assert ((eager.out[at:at + r].double() - want).abs() <= tol).all(), (rows, b)
+            at += r
+
+
+@pytest.mark.parametrize("lens", [[130, 69, 1], [200, 70, 1]])  # (the second: tokens that were never appended lie before the rows, NaN)
+def test_two_streams_of_portions_at_once(lens):
+    both, alone = [Prompts(BF16, i) for i in (1, 2)], [Prompts(BF16, i) for i in (1, 2)]
+    for p, o in zip(both, alone):
+        o.cache.page_table.copy_(p.cache.page_table)
+        for x in (p, o):
+            x.lens.copy_(i32(lens))
+            x.start.copy_(starts([130, 69, 1]))
+    for p in alone:
+        p.call()
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, s in zip(both, streams):
+            with torch.cuda.stream(s):
+                p.call()
+    torch.cuda.synchronize()
+    for p, o in zip(both, alone):
+        assert torch.isnan(p.out).any() == (lens[0] > 130) and torch.equal(p.out.view(torch.int16), o.out.view(torch.int16))

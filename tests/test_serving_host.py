@@ -90,6 +90,10 @@ def test_token_logprobs_is_checked(kw, text):
     refused(logprobs(**kw), text)
 
 
+def test_rows_of_all_heads_are_numbered_with_31_bits():
+    refused(attention(rows=1 << 30, start=P, heads=4), "too many for one call")
+
+
 def test_calls_without_rows_do_nothing():
     assert append(rows=0, start=P) == N.PG_OK and attention(rows=0, start=P) == N.PG_OK and logprobs(rows=0) == N.PG_OK
 
