@@ -9,7 +9,7 @@
 namespace pg {
 
 constexpr int KV8_MAX_SEQS = 4096;
-constexpr int KV8_STEP_ROWS = 64;
+constexpr int KV8_STEP_ROWS = 48;
 constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace does not hang on the device
 
 __host__ __device__ inline int kv8_padded(int head_dim) { return (head_dim + 63) / 64 * 64; }
