@@ -7,8 +7,8 @@
 // so both are K-major as they come. Four softmax warps for each tile have a row for every thread, which needs no exchange between
 // threads; one warp issues the products, the scores of a piece in front of the values of the one before it, so that the tensor pipe
 // works while the softmax of the next scores is computed. Two tiles share the producers' work at head_dim 128 (1500 rows behind 2600
-// positions, 32 query heads: 233 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are better (1000
-// rows of four sequences, 12 heads: 42 us, 55 us), above 128 tensor memory has room for one.
+// positions of two sequences, 32 query heads: 236 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are
+// better (1000 rows of four sequences, 12 heads: 41 us, 55 us), above 128 tensor memory has room for one.
 // Where the tiles are too few for the chip, each is cut along the positions (grid y); the parts, FP32 with their maxima and sums, are
 // merged by a kernel of their own in the order of the positions.
 //
@@ -32,7 +32,7 @@ template <int DP, typename T>
 struct PortionShape {
   static constexpr bool PAIR = std::is_same<T, float>::value;
   static constexpr int KC = DP / 64, TILES = DP == 128 ? 2 : 1;
-  static constexpr int PRODUCER_WARPS = DP == 64 ? 3 : 4;  // (3: eight warps in all, which leaves two CTAs 128 registers a thread)
+  static constexpr int PRODUCER_WARPS = DP == 64 ? 3 : DP == 128 ? 4 : 8;  // (3: eight warps in all, which leaves two CTAs 128 registers a thread)
   static constexpr int SOFTMAX_WARPS = TILES * TILE_WARPS, THREADS = (SOFTMAX_WARPS + 1 + PRODUCER_WARPS) * 32;
   static constexpr int TILE_QUERIES = (PAIR ? 2 : 1) * KC * 16384, QUERIES = TILES * TILE_QUERIES, HALF = KC * 8192, STAGE = 2 * HALF;  // bytes
   static constexpr int STAGES = QUERIES + 3 * STAGE <= (DP == 64 ? 100 : 192) * 1024 ? 3 : QUERIES + 2 * STAGE <= 192 * 1024 ? 2 : 1;
@@ -78,6 +78,54 @@ __device__ __forceinline__ bool elected() {
   return p != 0;
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A warp's 32 rows of COLS sums out of tensor memory, times a factor for each, to rows of `dim` entries at to(row) (null: none). A thread has
+// a row there, and neighbouring threads get neighbouring 16 bytes of one here: through shared memory (32 * COLS * sizeof(E) bytes). Where
+// there are no sums (any = false) the rows get `fill`, and that memory, which may still be in use, is left alone.
+template <typename E, int COLS, typename F>
+__device__ __forceinline__ void rows_out(uint8_t* mine, uint32_t taddr, bool any, float fill, float by, int dim, bool wide, F to) {
+  constexpr int PER = 16 / sizeof(E), VECS = COLS / PER;
+  static_assert(VECS % 8 == 0, "places are swapped among eight");
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int d = 0; d < COLS && any; d += 16) {
+    float o[16];
+    tmem_ld16(taddr + d, o);
+    union {
+      uint4 u[16 / PER];
+      E t[16];
+    } x;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x.t[e] = from_f32<E>(o[e] * by);
+#pragma unroll
+    for (int k = 0; k < 16 / PER; ++k) *reinterpret_cast<uint4*>(mine + (lane * VECS + ((d / PER + k) ^ (lane & 7))) * 16) = x.u[k];
+  }
+  __syncwarp();
+#pragma unroll 4
+  for (int k = lane; k < 32 * VECS; k += 32) {  // (all lanes as often: to() may exchange)
+    const int row = k / VECS, d = (k - row * VECS) * PER;
+    E* p = to(row);
+    if (!p) continue;
+    union {
+      uint4 u;
+      E t[PER];
+    } x;
+    if (any) {
+      x.u = *reinterpret_cast<const uint4*>(mine + (row * VECS + ((d / PER) ^ (row & 7))) * 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x.t[e] = from_f32<E>(fill);
+    }
+    if (wide && d + PER <= dim) {
+      *reinterpret_cast<uint4*>(p + d) = x.u;
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (d + e < dim) p[d + e] = x.t[e];
+    }
+  }
+  __syncwarp();
+}
 
 // Rows of one CTA (slot) and the pieces of 64 positions that they see: [0, kept) and [low, high). A sequence has the slots from
 // floor(its first row * group / size) + its number on; the last rows, which see most, come first.
@@ -168,37 +216,42 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
     // ---- a row for every thread
     const int tile = warp / TILE_WARPS, in_tile = tid & (ROWS - 1);
     const bool used = tile < tiles;
-    const int i = tile * ROWS + in_tile, x = row0 + min(i, rows - 1), tok = x / a.group, g = x - tok * a.group;
-    const int pos = len - r.n + tok;
+    const int i = tile * ROWS + in_tile, own = row0 + min(i, rows - 1), tok = own / a.group, pos = len - r.n + tok;
+    const int64_t entry = (int64_t)(head * a.group + own - tok * a.group) * c.dim;  // of the thread's own row, behind its token's first
+    auto wide_of = [&](const void* p, int64_t row) {
+      return (((uintptr_t)p | (uintptr_t)(row * (int64_t)sizeof(T)) | (uintptr_t)(c.dim * sizeof(T))) & 15) == 0;
+    };
+    const bool wide_rows = wide_of(a.q, a.q_row);
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tmem_o = o_of(tile) + lane_addr, tmem_s = tmem_o + DP;
     float back = 0.f;
     if (used) {
-      const T* q = (const T*)a.q + (size_t)(r.first + tok) * a.q_row + (size_t)(head * a.group + g) * c.dim;
-      const bool wide = c.dim % 8 == 0 && ((uintptr_t)q & 15) == 0;
-      auto eight = [&](int d, float (&v)[8]) {
-        if (wide && d + 8 <= c.dim) {
-          load8(q + d, v);
+      // a warp has 32 rows; neighbouring lanes take 8 entries each of the same one, so that it comes in whole lines
+      constexpr int ACROSS = DP == 64 ? 8 : DP == 128 ? 16 : 32, AT_ONCE = 32 / ACROSS;  // lanes for a row, rows at a time
+      const int u = lane % ACROSS;
+      const int64_t from = (int64_t)(r.first + tok) * a.q_row + entry;
+#pragma unroll 4
+      for (int k = 0; k < 32; k += AT_ONCE) {
+        const int row = (warp & 3) * 32 + k + lane / ACROSS;
+        const T* q = (const T*)a.q + __shfl_sync(ALL_LANES, from, k + lane / ACROSS) + u * 8;
+        float v[8], top = 0.f;
+        if (wide_rows && u * 8 + 8 <= c.dim) {
+          load8(q, v);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = d + e < c.dim ? to_f32(q[d + e]) : 0.f;
+          for (int e = 0; e < 8; ++e) v[e] = u * 8 + e < c.dim ? to_f32(q[e]) : 0.f;
         }
-      };
-      float top = 0.f;
-      for (int d = 0; d < c.dim; d += 8) {
-        float v[8];
-        eight(d, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-      }
-      // the sign of the score's factor goes to the queries, so that the largest product is the largest score
-      const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
-      const float f = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), a.scale);
-      back = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23), 1e-37f);  // never 0: a masked score is infinite
-      for (int u = 0; u < DP / 8; ++u) {  // 16 bytes each
-        float v[8];
-        eight(u * 8, v);
-        uint8_t* to = base + tile * S::TILE_QUERIES + (u >> 3) * 16384 + in_tile * 128 + (((u & 7) ^ (in_tile & 7)) << 4);
+#pragma unroll
+        for (int o = 1; o < ACROSS; o <<= 1) top = fmaxf(top, __shfl_xor_sync(ALL_LANES, top, o));
+        // the sign of the score's factor goes to the queries, so that the largest product is the largest score
+        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
+        const float f = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), a.scale);
+        const int mine = __shfl_sync(ALL_LANES, ex, lane % AT_ONCE * ACROSS);  // of this thread's own row
+        if (k == lane / AT_ONCE * AT_ONCE) back = __uint_as_float((uint32_t)(127 + mine) << 23);
+        if (u >= DP / 8) continue;
+        uint8_t* to = base + tile * S::TILE_QUERIES + (u >> 3) * 16384 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
         uint32_t h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -209,6 +262,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
         if (PAIR) *reinterpret_cast<uint4*>(to + KC * 16384) = make_uint4(l[0], l[1], l[2], l[3]);
       }
+      back = fmaxf(fabsf(a.scale) * 1.4426950408889634f * back, 1e-37f);  // never 0: a masked score is infinite
       fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[tile]);
@@ -303,41 +357,23 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
     if (ok && used && pieces > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (pieces - 1) & 1, failed, nullptr, 0));
     if (used) {
       tc_fence_after();
-      const bool part = w.parts > 1;
-      if (!ok) sum = __uint_as_float(0x7FC00000u);  // a wait ran out: no result, and one that shows
-      const float by = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-      T* out = (T*)a.out + (size_t)(r.first + tok) * a.out_row + (size_t)(head * a.group + g) * c.dim;
-      float* to = a.partials + (((size_t)blockIdx.x * gridDim.y + blockIdx.y) * (TILES * ROWS) + i) * (DP + 2);
-      if (part && i < rows) *reinterpret_cast<float2*>(to + DP) = make_float2(m_ref, sum);
-      const bool wide_out = c.dim % 8 == 0 && ((uintptr_t)out & 15) == 0;
+      const float fill = ok ? 0.f : __uint_as_float(0x7FC00000u);  // a wait ran out: no result, and one that shows
+      sum += fill;
+      uint8_t* mine = base + tile * S::TILE_QUERIES + (warp & 3) * (S::TILE_QUERIES / 4);  // the queries are not needed any more
+      const int row_w = tile * ROWS + (warp & 3) * 32;  // the warp's first row
+      const bool any = pieces > 0 && ok;
+      if (w.parts > 1) {
+        float* to = a.partials + ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * (TILES * ROWS) * (DP + 2);
+        if (i < rows) *reinterpret_cast<float2*>(to + (size_t)TILES * ROWS * DP + 2 * i) = make_float2(m_ref, sum);
 #pragma unroll 1
-      for (int d = 0; d < c.dim; d += 16) {
-        float o[16];
-        if (pieces > 0 && ok) {
-          tmem_ld16(tmem_o + d, o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = 0.f;
-        }
-        if (i < rows && part) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) *reinterpret_cast<float2*>(to + d + e) = make_float2(o[e], o[e + 1]);
-        } else if (i < rows) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] *= by;
-#pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            if (wide_out && d + e + 8 <= c.dim) {
-              store4(out + d + e, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
-              store4(out + d + e + 4, make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (d + e + k < c.dim) out[d + e + k] = from_f32<T>(o[e + k]);
-            }
-          }
-        }
-        __syncwarp();
+        for (int d = 0; d < DP; d += DP / 2)
+          rows_out<float, DP / 2>(mine, tmem_o + d, any, fill, 1.f, DP / 2, true, [&](int k) { return row_w + k < rows ? to + (row_w + k) * DP + d : nullptr; });
+      } else {
+        const int64_t at = (int64_t)(r.first + tok) * a.out_row + entry;
+        rows_out<T, DP>(mine, tmem_o, any, fill, sum == 0.f ? 0.f : 1.f / sum, c.dim, wide_of(a.out, a.out_row), [&](int k) {
+          T* p = (T*)a.out + __shfl_sync(ALL_LANES, at, k);
+          return row_w + k < rows ? p : nullptr;
+        });
       }
     }
     tc_fence_before();
@@ -503,10 +539,10 @@ __global__ void __launch_bounds__(128) kv8_portion_merge_kernel(Kv8AttnArgs a, i
   const Portion w(a, slot, SIZE, most_parts);
   const int i = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (i >= w.rows || w.parts <= 1) return;
-  const float* from = a.partials + ((size_t)blockIdx.x * most_parts * SIZE + i) * (DP + 2);
+  const float* from = a.partials + (size_t)blockIdx.x * most_parts * SIZE * (DP + 2) + (size_t)i * DP;
   const size_t step = (size_t)SIZE * (DP + 2);
   // a lane for a part (at most 32): its maximum, what it is to be multiplied with
-  const float2 ml = lane < w.parts ? *reinterpret_cast<const float2*>(from + lane * step + DP) : make_float2(-INFINITY, 0.f);
+  const float2 ml = lane < w.parts ? *reinterpret_cast<const float2*>(from + lane * step + (size_t)(SIZE - i) * DP + 2 * i) : make_float2(-INFINITY, 0.f);
   const float top = lane_max(ml.x), f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - top), sum = lane_sum(ml.y * f);
   const float by = sum == 0.f ? 0.f : 1.f / sum;
   const int x = w.row0 + i, tok = x / a.group;
