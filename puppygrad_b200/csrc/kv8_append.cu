@@ -8,7 +8,9 @@
 //  - one token for every sequence: a warp for each block and each query head, an entry for every lane;
 //  - more, rows on 16-byte boundaries: a CTA for each block, eight entries for a thread at a time, in registers;
 //  - more, any rows: a CTA for each block, values staged in shared memory.
-// Bound: memory (every value read once, every code written once); a step of few tokens is launch latency.
+// Bound: memory (every value read once, every code written once); a step of few tokens is launch latency. Measured: 8 prompts of up to 2047
+// tokens, 52 us (21 by bytes: instructions of the conversions, and a block's loads, maximum and stores one after the other); 64 single tokens
+// 4.8 us, one 2.2 us.
 #include "kv8.cuh"
 
 namespace pg {

@@ -14,6 +14,8 @@
 // A group's sums are FP32, times the scale once per 64 inputs.
 // A CTA has a range of the tiles of 16 outputs and goes over it in passes of up to R tiles, so that 64 inputs once loaded serve R tiles. Its
 // warps take every WARPS-th tile of 64 inputs and are added up in shared memory, in order.
+// Measured: 28672 x 8192, 8 rows 38 us (3.2 TB/s), 16 rows 48 us, 19 us by bytes: taking the codes apart and the matrix instructions are
+// what an SM is busy with. 2304 x 768, one row: 2.6 us, a launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -295,7 +297,8 @@ struct Variant {
   }
 };
 // Few tiles of outputs for a CTA: 16 warps share the inputs' length, which is latency. Many: 8 warps, whose registers hold more tiles, so
-// that what is done once for 64 inputs serves more outputs.
+// that what is done once for 64 inputs serves more outputs. us with few / many, 8 rows: 2304 x 768 FP32 2.6 / 3.3, 6400 x 1600 BF16 3.8 / 4.8,
+// 28672 x 8192 BF16 40 / 38. (Weights through a ring of shared memory, bulk copies: as fast as these loads into registers, 37 to 39.)
 template <typename T, int NT>
 struct Choice {
   static constexpr bool PAIR = std::is_same<T, float>::value;

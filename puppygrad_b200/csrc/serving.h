@@ -9,7 +9,10 @@
 namespace pg {
 
 constexpr int KV8_MAX_SEQS = 4096;
-constexpr int KV8_STEP_ROWS = 48;
+// Rows of a (sequence, head) up to which the step kernel has them. us, step / portion kernel, at 32, 48 and 64 rows: 16 sequences of 2000
+// positions, 8 heads of 128, BF16 49 / 51, 65 / 50, 77 / 50, FP32 76 / 71, 104 / 72, 131 / 72; 64 of them BF16 140 / 229, 197 / 232, 254 / 261, FP32
+// 269 / 290, 387 / 302, 513 / 312; 12 heads of 64 BF16 137 / 180, 176 / 185, 241 / 201; 8 of 4000, 4 heads of 256, BF16 64 / 59, 88 / 69, 106 / 70.
+constexpr int KV8_STEP_ROWS = 40;
 constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace does not hang on the device
 
 __host__ __device__ inline int kv8_padded(int head_dim) { return (head_dim + 63) / 64 * 64; }
