@@ -9,7 +9,7 @@
 //  - more, rows on 16-byte boundaries: a CTA for each block, eight entries for a thread at a time, in registers;
 //  - more, any rows: a CTA for each block, values staged in shared memory.
 // Bound: memory (every value read once, every code written once); a step of few tokens is launch latency. Measured: 8 prompts of up to 2047
-// tokens, 52 us (21 by bytes: instructions of the conversions, and a block's loads, maximum and stores one after the other); 64 single tokens
+// tokens, 46 us (21 by bytes: instructions of the conversions, and a block's loads, maximum and stores one after the other); 64 single tokens
 // 4.8 us, one 2.2 us.
 #include "kv8.cuh"
 
@@ -236,8 +236,41 @@ __global__ void __launch_bounds__(THREADS, DP <= 128 ? 4 : 2) kv8_append_block_k
   grid_dep_wait();
   const Kv8View& c = a.c;
   const int tid = threadIdx.x, blocks = slots * c.kv_heads * 2, dim = c.dim;
-  if ((int)blockIdx.x >= blocks) {
-    const int row0 = ((int)blockIdx.x - blocks) * QUERY_ROWS, n = min(QUERY_ROWS, a.rows - row0), half = a.rot_dims >> 1;
+  // CTAs of blocks, which compute more, and of queries, which move more, in turn
+  const int both = min(blocks, (int)gridDim.x - blocks), bx = blockIdx.x;
+  const bool queries = bx < 2 * both ? bx & 1 : blocks == both;
+  const int number = bx < 2 * both ? bx >> 1 : bx - both;
+  if (queries) {
+    const int row0 = number * QUERY_ROWS, n = min(QUERY_ROWS, a.rows - row0), half = a.rot_dims >> 1;
+    // an item: entries 8 i .. and their partners together (q_out may be q), of several rows, which are on their way at once; the first
+    // item's before the positions are known
+    constexpr int AT_ONCE = sizeof(T) == 2 ? 4 : 2, VECS = sizeof(T) / 2;  // rows; 16-byte words of 8 values
+    const int pairs = half >> 3, per = pairs + ((dim - 2 * half) >> 3), across = a.heads * per, items = across * ((n + AT_ONCE - 1) / AT_ONCE);
+    uint4 u[AT_ONCE][VECS], w[AT_ONCE][VECS];
+    struct Item {
+      int t0, i;
+      int64_t at;
+    };
+    auto item_at = [&](int y) {
+      const int t = y / across, x = y - t * across, h = x / per, i = x - h * per;
+      return Item{t * AT_ONCE, i, (int64_t)h * dim + (i < pairs ? i * 8 : 2 * half + (i - pairs) * 8)};
+    };
+    auto ask = [&](const Item& m) {
+      const T* q = (const T*)a.q + row0 * a.q_row + m.at;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (m.t0 + k < n)
+#pragma unroll
+          for (int e = 0; e < VECS; ++e) {
+            u[k][e] = reinterpret_cast<const uint4*>(q + (m.t0 + k) * a.q_row)[e];
+            if (m.i < pairs) w[k][e] = reinterpret_cast<const uint4*>(q + (m.t0 + k) * a.q_row + half)[e];
+          }
+    };
+    Item m{};
+    if (tid < items) {
+      m = item_at(tid);
+      ask(m);
+    }
     if (tid < n) {
       bool any;
       positions[tid] = row_position(a, row0 + tid, &any);
@@ -245,49 +278,35 @@ __global__ void __launch_bounds__(THREADS, DP <= 128 ? 4 : 2) kv8_append_block_k
     }
     __syncthreads();
     turn_table_by_eights(a, turns, cs, n, half, 0, positions);
-    // entries 8 i .. and their partners together (q_out may be q), those of several rows on their way at once
-    constexpr int AT_ONCE = sizeof(T) == 2 ? 4 : 2, VECS = sizeof(T) / 2;  // 16-byte words of 8 values
-    const int pairs = half >> 3, per = pairs + ((dim - 2 * half) >> 3);
-    for (int y = tid; y < a.heads * per; y += THREADS) {
-      const int h = y / per, i = y - h * per;
-      const bool pair = i < pairs;
-      const int64_t at = (int64_t)h * dim + (pair ? i * 8 : 2 * half + (i - pairs) * 8);
-      const T* q = (const T*)a.q + row0 * a.q_row + at;
-      T* o = (T*)a.q_out + row0 * a.q_out_row + at;
-      for (int t0 = 0; t0 < n; t0 += AT_ONCE) {
-        uint4 u[AT_ONCE][VECS], w[AT_ONCE][VECS];
+    for (int y = tid; y < items; y += THREADS) {
+      if (y != tid) {
+        m = item_at(y);
+        ask(m);
+      }
+      T* o = (T*)a.q_out + row0 * a.q_out_row + m.at;
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k)
-          if (t0 + k < n)
+      for (int k = 0; k < AT_ONCE; ++k) {
+        if (m.t0 + k >= n || !there[m.t0 + k]) continue;
+        T* to = o + (m.t0 + k) * a.q_out_row;
+        if (m.i < pairs) {
+          float f[8], g[8];
+          load8(reinterpret_cast<const T*>(u[k]), f);
+          load8(reinterpret_cast<const T*>(w[k]), g);
+          turn_eight(cs, m.t0 + k, pairs, m.i, f, g);
+          store4(to, make_float4(f[0], f[1], f[2], f[3]));
+          store4(to + 4, make_float4(f[4], f[5], f[6], f[7]));
+          store4(to + half, make_float4(g[0], g[1], g[2], g[3]));
+          store4(to + half + 4, make_float4(g[4], g[5], g[6], g[7]));
+        } else {
 #pragma unroll
-            for (int e = 0; e < VECS; ++e) {
-              u[k][e] = reinterpret_cast<const uint4*>(q + (t0 + k) * a.q_row)[e];
-              if (pair) w[k][e] = reinterpret_cast<const uint4*>(q + (t0 + k) * a.q_row + half)[e];
-            }
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) {
-          if (t0 + k >= n || !there[t0 + k]) continue;
-          T* to = o + (t0 + k) * a.q_out_row;
-          if (pair) {
-            float f[8], g[8];
-            load8(reinterpret_cast<const T*>(u[k]), f);
-            load8(reinterpret_cast<const T*>(w[k]), g);
-            turn_eight(cs, t0 + k, pairs, i, f, g);
-            store4(to, make_float4(f[0], f[1], f[2], f[3]));
-            store4(to + 4, make_float4(f[4], f[5], f[6], f[7]));
-            store4(to + half, make_float4(g[0], g[1], g[2], g[3]));
-            store4(to + half + 4, make_float4(g[4], g[5], g[6], g[7]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < VECS; ++e) reinterpret_cast<uint4*>(to)[e] = u[k][e];
-          }
+          for (int e = 0; e < VECS; ++e) reinterpret_cast<uint4*>(to)[e] = u[k][e];
         }
       }
     }
     return;
   }
-  const int side = blockIdx.x & 1, h = (blockIdx.x >> 1) % c.kv_heads;
-  const PageRows pr(a, (blockIdx.x >> 1) / c.kv_heads);
+  const int side = number & 1, h = (number >> 1) % c.kv_heads;
+  const PageRows pr(a, (number >> 1) / c.kv_heads);
   if (pr.page < 0) return;
   const int p = c.page_tokens, half = side == 0 ? a.rot_dims >> 1 : 0, n = pr.n, o0 = pr.o0;
   if (half) turn_table_by_eights(a, turns, cs, n, half, pr.pos0, nullptr);
