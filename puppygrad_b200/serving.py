@@ -42,6 +42,13 @@ def _device(t, name: str) -> int:
     return device
 
 
+def _sides(t, name: str, n: int):
+    """Shape of a buffer that has to have n dimensions."""
+    if len(t.shape) != n:
+        raise _bad(f"{name} {tuple(t.shape)} must have {n} dimensions")
+    return t.shape
+
+
 def _flat(t, name: str, dtype: str, shape: Tuple[int, ...], device: int) -> int:
     """Address of a buffer that has to be contiguous and of that type and shape."""
     if t.shape == shape and _seen.get(t.dtype) == dtype and t.is_contiguous() and t.get_device() == device:
@@ -77,9 +84,8 @@ class Kv8Cache:
 
     def __init__(self, pool, scales, page_table, page_tokens: int, head_dim: int):
         device = _device(pool, "pool")
-        if len(pool.shape) != 3 or len(page_table.shape) != 2:
-            raise _bad(f"pool {tuple(pool.shape)} and page_table {tuple(page_table.shape)} must have 3 and 2 dimensions")
-        n_pages, kv_heads = pool.shape[:2]
+        _sides(page_table, "page_table", 2)
+        n_pages, kv_heads = _sides(pool, "pool", 3)[:2]
         self._c = N.PgKv8Cache()
         self._c.pool = _flat(pool, "pool", "torch.uint8", self.pool_shape(n_pages, kv_heads, page_tokens, head_dim), device)
         self._c.scales = _flat(scales, "scales", "torch.float32", (n_pages, kv_heads, 2), device)
@@ -101,7 +107,7 @@ class Kv8Cache:
         """Appends k and v [rows, kv_heads, head_dim], k turned by its positions; q [rows, heads, head_dim] is turned into q_out (which
         may be q). Sequence b has rows row_start[b] : row_start[b + 1] (None: row b), at the last positions of lens[b], its
         length with them."""
-        rows, device, kind = k.shape[0], self.device, k.dtype
+        rows, device, kind = _sides(k, "k", 3)[0], self.device, k.dtype
         dtype, shape = _code(k, "k"), (rows, self.kv_heads, self.head_dim)
         kp, ks = _rows(k, "k", kind, shape, device)
         vp, vs = _rows(v, "v", kind, shape, device)
@@ -109,7 +115,7 @@ class Kv8Cache:
         if q is not None or q_out is not None:
             if q is None or q_out is None:
                 raise _bad("q and q_out must be given together")
-            heads = q.shape[1]
+            heads = _sides(q, "q", 3)[1]
             shape = (rows, heads, self.head_dim)
             qp, qs = _rows(q, "q", kind, shape, device)
             op, os = _rows(q_out, "q_out", kind, shape, device)
@@ -132,14 +138,14 @@ class Kv8Cache:
         """out = softmax(scale * q . k) v over what each row sees; q and out [rows, heads, head_dim], scale head_dim ** -0.5 unless
         given, `lens` and `row_start` as in `append`. max_rows: at least the rows of any sequence. `workspace`: uint8, zeroed
         before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each."""
-        device, kind, shape = self.device, q.dtype, (*q.shape[:2], self.head_dim)
+        device, kind, shape = self.device, q.dtype, (*_sides(q, "q", 3)[:2], self.head_dim)
         rows, heads = shape[:2]
         dtype = _code(q, "q")
         qp, qs = _rows(q, "q", kind, shape, device)
         op, os = _rows(out, "out", kind, shape, device)
         lp = _flat(lens, "lens", "torch.int32", (self.seqs,), device)
         sp = 0 if row_start is None else _flat(row_start, "row_start", "torch.int32", (self.seqs + 1,), device)
-        size = workspace.shape[0]
+        size = _sides(workspace, "workspace", 1)[0]
         wp = _flat(workspace, "workspace", "torch.uint8", (size,), device)
         status = N.lib.pg_kv8_attention(self._ref, qp, qs, op, os, dtype, heads, rows, max_rows, sp, lp,
                                         self.head_dim ** -0.5 if scale is None else scale, window, keep_first, wp, size, stream)
@@ -156,7 +162,7 @@ def q4_shapes(n: int, k: int, group: int) -> Tuple[Tuple[int, int, int], Tuple[i
 
 def quantize_q4(w, packed, scales, group: int, stream: int = 0) -> None:
     """Lays the matrix w [n, k] out in 4 bits, with one scale for every `group` (64 or 128) inputs of an output."""
-    n, k = w.shape
+    n, k = _sides(w, "w", 2)
     dtype, device = _code(w, "w"), _device(w, "w")
     wp, ws = _rows(w, "w", w.dtype, (n, k), device)
     ps, ss = q4_shapes(n, k, group)
@@ -166,8 +172,8 @@ def quantize_q4(w, packed, scales, group: int, stream: int = 0) -> None:
 
 def linear_q4(x, packed, scales, out, group: int, bias=None, stream: int = 0) -> None:
     """out [m, n] = x [m, k] @ dequant(w [n, k]).T + bias for up to 16 rows."""
-    m, k = x.shape
-    n, kind = out.shape[1], x.dtype
+    m, k = _sides(x, "x", 2)
+    n, kind = _sides(out, "out", 2)[1], x.dtype
     dtype, device = _code(x, "x"), _device(x, "x")
     xp, xs = _rows(x, "x", kind, (m, k), device)
     op, os = _rows(out, "out", kind, (m, n), device)
@@ -183,7 +189,7 @@ def linear_q4(x, packed, scales, out, group: int, bias=None, stream: int = 0) ->
 def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=None, top_logprobs=None, stream: int = 0) -> None:
     """Scores of the rows of logits [rows, vocab]: logprobs [rows] of `targets` [rows], entropy [rows], the most likely ids and their
     log probabilities [rows, k] (k up to 32), each where its output is given."""
-    rows, vocab = logits.shape
+    rows, vocab = _sides(logits, "logits", 2)
     dtype, device, each = _code(logits, "logits"), _device(logits, "logits"), (rows,)
     lp, ls = _rows(logits, "logits", logits.dtype, (rows, vocab), device)
     if (top_ids is None) != (top_logprobs is None):
@@ -193,7 +199,7 @@ def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=No
     ep = 0 if entropy is None else _flat(entropy, "entropy", "torch.float32", each, device)
     k = ip = vp = 0
     if top_ids is not None:
-        k = top_ids.shape[1]
+        k = _sides(top_ids, "top_ids", 2)[1]
         ip = _flat(top_ids, "top_ids", "torch.int32", (rows, k), device)
         vp = _flat(top_logprobs, "top_logprobs", "torch.float32", (rows, k), device)
     status = N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, tp, op, ep, k, ip, vp, device, stream)

@@ -121,3 +121,10 @@ def test_tensors_on_the_host_are_refused():
         pg.token_logprobs(x.double(), entropy=torch.zeros(2))
     with pytest.raises(pg.Gpt2Error, match="a CUDA device is needed"):
         pg.Kv8Cache(x, x, x, page_tokens=16, head_dim=64)
+
+
+def test_buffers_with_another_number_of_dimensions_are_refused():
+    x, y = torch.zeros(5), torch.zeros(2, 5)
+    for call in (lambda: pg.token_logprobs(x), lambda: pg.linear_q4(x, y, y, y, 64), lambda: pg.linear_q4(y, y, y, x, 64), lambda: pg.quantize_q4(x, y, y, 64)):
+        with pytest.raises(pg.Gpt2Error, match=r"\(5,\) must have 2 dimensions"):
+            call()
