@@ -14,8 +14,9 @@
 // A group's sums are FP32, times the scale once per 64 inputs.
 // A CTA has a range of the tiles of 16 outputs and goes over it in passes of up to R tiles, so that 64 inputs once loaded serve R tiles. Its
 // warps take every WARPS-th tile of 64 inputs and are added up in shared memory, in order.
-// Measured: 28672 x 8192, 8 rows 38 us (3.2 TB/s), 16 rows 48 us, 19 us by bytes: taking the codes apart and the matrix instructions are
-// what an SM is busy with. 2304 x 768, one row: 2.6 us, a launch.
+// Measured: 28672 x 8192, 8 rows 38 us (3.2 TB/s), 16 rows 48 us, 19 us by bytes: two warps a scheduler, whose chains of shifts, masks
+// and matrix instructions leave half of the cycles free; more warps with fewer registers were slower (45 to 55). 2304 x 768, one row:
+// 2.6 us, a launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
