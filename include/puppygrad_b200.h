@@ -388,7 +388,8 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
  * (it chooses the kernels; a sequence with more is still computed). Where row_start decreases, rows are left out or computed twice. FP32 queries are computed to FP32 grade from pairs of
  * FP16 numbers, BF16 queries with FP16 probabilities; sums are FP32.
  * workspace: pg_kv8_attention_workspace_bytes() bytes, 256-byte aligned, zeroed by the caller before its first use and left ready for the next
- * call. Calls that may overlap on the GPU (captured graphs among them) need workspaces of their own. */
+ * call, whatever that one's cache, rows, heads and type are, as long as the workspace has the bytes it needs. Calls that may overlap on the
+ * GPU (captured graphs among them) need workspaces of their own. */
 uint64_t pg_kv8_attention_workspace_bytes(const pg_kv8_cache* cache, int32_t rows, int32_t heads, int32_t dtype);
 int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, void* out, int64_t out_row, int32_t dtype,
                      int32_t heads, int32_t rows, int32_t max_rows, const int32_t* row_start, const int32_t* lens, float scale,

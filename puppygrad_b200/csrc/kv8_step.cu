@@ -127,7 +127,7 @@ struct Sixteen {
 
 // A tile of rows, and where its units lie among all units.
 struct Tile {
-  int b, head, row0, rows, first_row, n_rows, len, have, first_unit, units, counter;
+  int b, head, row0, rows, first_row, n_rows, len, have, first_unit, units;
   Span span;
 };
 // Equal shares of the units: share i begins at floor(i * units / n), without 64-bit divisions. Shares of equal tiles begin where
@@ -249,7 +249,6 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
     const int tile = x - t.head * tiles;
     t.row0 = tile * ROWS;
     t.rows = min(ROWS, r.n * a.group - t.row0);
-    t.counter = ((int)((int64_t)r.first * a.group / ROWS) + t.b + tile) * c.kv_heads + t.head;
     return t;
   };
   auto start_of = [&](const Span& s, int x) { return (x < s.keep ? x : s.low + x - s.keep) * UNIT; };
@@ -641,7 +640,8 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        unsigned* counter = a.counters + t.counter;
+        // that of the CTA in which the tile begins; no other tile reaches from there into the next one
+        unsigned* counter = a.counters + first_cta;
         const bool last = atomicAdd(counter, 1u) == (unsigned)(n - 1);
         if (last) *counter = 0;  // ready for the next call
         __threadfence();

@@ -108,12 +108,11 @@ Kv8View view(const pg_kv8_cache* c) {
           c->kv_heads, c->head_dim, c->seqs, c->pages_per_seq};
 }
 
-// Counters of the step kernel, one for each tile of (at least 8) rows that several CTAs may share, then parts of tiles: two for every
-// CTA and one for each of its warps, of which there are 16 with tiles of 8 rows, 8 with tiles of 16.
-size_t counter_bytes(const pg_kv8_cache* c, int rows, int heads) {
-  const int64_t tiles = ((int64_t)rows * (heads / c->kv_heads) / 8 + c->seqs) * c->kv_heads;
-  return ((size_t)tiles * 4 + 255) / 256 * 256;
-}
+// A workspace: counters of the step kernel, one for each of its CTAs, then parts of tiles: two for every CTA and one for each of its warps, of
+// which there are 16 with tiles of 8 rows, 8 with tiles of 16. Where the counters lie is the same for all calls: parts that one call
+// leaves are never what the next one counts with.
+constexpr size_t COUNTER_BYTES = 1024;
+static_assert(COUNTER_BYTES >= KV8_MAX_CTAS * 4, "a counter for each CTA");
 size_t partial_bytes(const pg_kv8_cache* c) {
   const int padded = kv8_padded(c->head_dim), rows = padded == 64 ? (2 + 16) * 16 : std::max((2 + 16) * 8, (2 + 8) * 16);
   // (the portion kernel, which runs behind the step kernel, cuts its tiles of 128 or 256 rows into as many parts)
@@ -163,7 +162,7 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
 uint64_t pg_kv8_attention_workspace_bytes(const pg_kv8_cache* cache, int32_t rows, int32_t heads, int32_t dtype) {
   if (check_cache(cache) || check_dtype(dtype) || check_heads(cache, heads)) return 0;
   if (rows < 0) return bad("rows must not be negative"), 0;
-  return counter_bytes(cache, rows, heads) + partial_bytes(cache);
+  return COUNTER_BYTES + partial_bytes(cache);
 }
 
 int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, void* out, int64_t out_row, int32_t dtype,
@@ -195,7 +194,7 @@ int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, vo
   // rows that fill less than half a tile of the portion kernel, and all of them where it has no table of rows
   const bool portions = row_start && (int64_t)group * max_rows > KV8_STEP_ROWS;
   Kv8AttnArgs a{view(cache), q, out, q_row, out_row, heads, group, rows, max_rows, row_start, lens, scale, window, window > 0 ? keep_first : 0,
-                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)workspace, (float*)((char*)workspace + counter_bytes(cache, rows, heads))};
+                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)workspace, (float*)((char*)workspace + COUNTER_BYTES)};
   if (!portions) return launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention");
   a.max_rows = std::min(max_rows, (KV8_STEP_ROWS + group - 1) / group);
   if (int r = launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention")) return r;

@@ -126,7 +126,8 @@ class Kv8Cache:
             check(status)
 
     def workspace_bytes(self, rows: int, heads: int, dtype) -> int:
-        """Size of the workspace of `attention` calls of up to that many rows; its memory must be zero before its first use."""
+        """Size of the workspace of `attention` calls of up to that many rows; its memory must be zero before its first use. Calls over
+        different caches, rows and heads can share one, one after the other, if it has the most bytes that any of them needs."""
         code = _CODES.get(_name(dtype), -1)
         size = N.lib.pg_kv8_attention_workspace_bytes(self._ref, rows, heads, code)
         if not size:

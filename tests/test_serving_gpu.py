@@ -819,3 +819,19 @@ def test_two_streams_of_portions_at_once(lens):
     torch.cuda.synchronize()
     for p, o in zip(both, alone):
         assert torch.isnan(p.out).any() == (lens[0] > 130) and torch.equal(p.out.view(torch.int16), o.out.view(torch.int16))
+
+
+# ------------------------------------------------------------------ one workspace, queries and inputs of every finite size, long tails
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_calls_of_all_sizes_share_a_workspace(dtype):
+    """Steps, mixed calls with more rows and calls over another cache, one after the other: whatever one leaves, the next gives all its rows."""
+    lens = [1600] + [100 + i * 53 % 900 for i in range(63)]
+    wide, small = Cache(lens, 8, 128, 64, 41), Cache([5000, 70, 3000], 1, 64, 16, 42)
+    size = max(wide.handle.workspace_bytes(2000, 32, dtype), small.handle.workspace_bytes(3, 8, dtype))
+    ws = torch.zeros(size, dtype=torch.uint8, device=DEV)
+    calls = [(wide, 32, [1] * 64), (wide, 32, [1500] + [1] * 63), (small, 8, [1] * 3), (wide, 32, [700] + [3] * 63), (wide, 32, [1] * 64), (small, 8, [1, 60, 2])]
+    for i, (cache, heads, rows) in enumerate(calls):
+        q = torch.randn(sum(rows), heads, cache.dim, generator=gen(i), device=DEV).to(dtype)
+        out = torch.full_like(q, 1e4)
+        cache.handle.attention(q, out, i32(cache.lens), ws, row_start=starts(rows), max_rows=max(rows))
+        check_attention(cache, q, out, rows, cache.dim ** -0.5)
