@@ -101,7 +101,8 @@ struct Operand<float> {
     for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
     m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 1));
     m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 2));
-    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
+    // exponents within +-126 keep both the factor and its inverse normal numbers, and the largest input, 2^128, below 4
+    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 126);
     const float s = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

@@ -835,3 +835,18 @@ def test_attention_calls_of_all_sizes_share_a_workspace(dtype):
         out = torch.full_like(q, 1e4)
         cache.handle.attention(q, out, i32(cache.lens), ws, row_start=starts(rows), max_rows=max(rows))
         check_attention(cache, q, out, rows, cache.dim ** -0.5)
+
+
+def test_linear_q4_inputs_at_the_ends_of_the_range():
+    n, k = 64, 256
+    ps, ss = pg.q4_shapes(n, k, 64)
+    packed, scales = torch.empty(ps, dtype=torch.uint8, device=DEV), torch.empty(ss, dtype=BF16, device=DEV)
+    pg.quantize_q4(torch.randn(n, k, generator=gen(1), device=DEV), packed, scales, 64)
+    w = ref.q4_weights(packed, scales, n, k, 64)
+    x = torch.randn(12, k, generator=gen(2), device=DEV)
+    x[0:4] *= 2.0 ** 116  # 64 magnitudes add up to 2^122
+    x[4:8] *= 2.0 ** -120
+    out = torch.empty(12, n, device=DEV)
+    pg.linear_q4(x, packed, scales, out, 64)
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    assert ((out.double() - want).abs() <= 2.0 ** -18 * size).all()
