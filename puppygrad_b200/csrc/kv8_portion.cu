@@ -251,7 +251,8 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
 #pragma unroll
         for (int o = 1; o < ACROSS; o <<= 1) top = fmaxf(top, __shfl_xor_sync(ALL_LANES, top, o));
         // the sign of the score's factor goes to the queries, so that the largest product is the largest score
-        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
+        // (exponents within +-126: both the factor and its inverse are normal numbers, and the largest entry, 2^128, becomes less than 4)
+        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
         const float f = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), a.scale);
         const int mine = __shfl_sync(ALL_LANES, ex, lane % AT_ONCE * ACROSS);  // of this thread's own row
         if (k == lane / AT_ONCE * AT_ONCE) back = __uint_as_float((uint32_t)(127 + mine) << 23);
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
         if (PAIR) *reinterpret_cast<uint4*>(to + KC * 16384) = make_uint4(l[0], l[1], l[2], l[3]);
       }
-      back = fmaxf(fabsf(a.scale) * 1.4426950408889634f * back, 1e-37f);  // never 0: a masked score is infinite
+      back = fabsf(a.scale) * 1.4426950408889634f * back;
       fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[tile]);

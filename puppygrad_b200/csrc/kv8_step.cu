@@ -338,8 +338,8 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
         }
       m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 1));
       m = fmaxf(m, __shfl_xor_sync(ALL_LANES, m, 2));
-      // exponents within +-100 keep both the factor and its inverse normal numbers
-      const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
+      // exponents within +-126 keep both the factor and its inverse normal numbers, and the largest entry, 2^128, below 4
+      const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 126);
       // the sign of the score's factor goes to the queries, so that the largest product is the largest score
       const float f = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), a.scale);
       const float b = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + ex) << 23);

@@ -850,3 +850,14 @@ def test_linear_q4_inputs_at_the_ends_of_the_range():
     pg.linear_q4(x, packed, scales, out, 64)
     want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
     assert ((out.double() - want).abs() <= 2.0 ** -18 * size).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 90])
+@pytest.mark.parametrize("size", [2.0 ** -120, 2.0 ** 120])
+def test_attention_queries_at_the_ends_of_the_range(size, rows, dtype):
+    cache = Cache([300], 1, 64, 16, 3)
+    q = (torch.randn(rows, 2, 64, generator=gen(1), device=DEV) * size).to(dtype)
+    out = torch.full_like(q, 1e4)
+    cache.handle.attention(q, out, i32([300]), workspace(cache, rows, 2, dtype), row_start=starts([rows]), max_rows=rows, scale=0.125 / size)
+    check_attention(cache, q, out, [rows], 0.125 / size)
