@@ -407,7 +407,7 @@ int pg_quantize_q4(const void* w, int64_t w_row, int32_t dtype, int32_t n, int32
                    int32_t device, void* stream);
 /* out[m][n] = x[m][k] . dequant(w)[n][k]^T + bias; 1 <= m <= 16; x, bias (may be NULL) and out FP32 or BF16. FP32 inputs are
  * computed to FP32 grade from pairs of FP16 numbers. A row with a NaN or an infinity gives NaN, one with 64 inputs whose magnitudes add
- * up to more than 2^124 (BF16: 2^120) NaN or infinities. */
+ * up to more than 2^124 NaN or infinities. */
 int pg_linear_q4(const void* x, int64_t x_row, const void* packed, const void* scales, const void* bias, int32_t dtype, int32_t m,
                  int32_t n, int32_t k, int32_t group, void* out, int64_t out_row, int32_t device, void* stream);
 

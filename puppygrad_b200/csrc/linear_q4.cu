@@ -5,18 +5,18 @@
 // instructions with 16 outputs as rows and 8 tokens as columns, on codes turned into 16-bit floats in registers. Order of k within a
 // tile is free as long as both operands agree: a lane takes 16 consecutive inputs (k steps of 4), so it loads 16 bytes of weights
 // (8 of outputs r and of r + 8) and 16 inputs in a row.
-//  - BF16 inputs are exact operands; a field of 4 bits or-ed into the mantissa of 128 is 128 + code. The accumulators start at -136 sum x
-//    instead of subtracting 136 from every weight, which one more product with a constant operand gives in their own layout, once
-//    for all the outputs of a pass.
+//  - Weights are exact: a field of 4 bits or-ed into the mantissa of a power of two, less what that adds. (Sums that start at -136 sum x
+//    in place of the subtraction are off by a part of the inputs' size even where the weights are zero.)
+//  - BF16 inputs are exact operands. A product with zeros, once for all the outputs of a pass, makes the sums of a row with a NaN or an infinity
+//    start at NaN.
 //  - FP32 inputs are pairs of FP16 numbers, scaled by a power of two for every 64 inputs of a row, the rests' products first, then the
-//    others' into the same accumulator, and exact weights: FP32 grade (the instruction cuts off sums, so that starting far from zero
-//    would show: 1.2e-6 where this is off by 1e-7).
+//    others' into the same accumulator: FP32 grade.
 // A group's sums are FP32, times the scale once per 64 inputs.
 // A CTA has a range of the tiles of 16 outputs and goes over it in passes of up to R tiles, so that 64 inputs once loaded serve R tiles. Its
 // warps take every WARPS-th tile of 64 inputs and are added up in shared memory, in order.
-// Measured: 28672 x 8192, 8 rows 38 us (3.2 TB/s), 16 rows 48 us, 19 us by bytes: two warps a scheduler, whose chains of shifts, masks
-// and matrix instructions leave half of the cycles free; more warps with fewer registers were slower (45 to 55). 2304 x 768, one row:
-// 2.6 us, a launch.
+// Measured: 28672 x 8192, BF16, 8 rows 42 us (3.0 TB/s), 16 rows 53 us, FP32 54 and 75 us, 19 us by bytes: two warps a scheduler, whose
+// chains of shifts, masks, subtractions and matrix instructions leave half of the cycles free. The subtraction is 4 and 5 us of the BF16 times; multiply-adds
+// that also save the shifts (fields in bits 4-7 taken as numbers below 2^-125) were slower, 59 us at 16 rows. 2304 x 768, one row: 2.2 us, a launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -41,8 +41,8 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Inputs 2 i and 2 i + 1 of a word of 8 codes as 16-bit floats: BF16 128 + code, FP16 the weight code - 8 itself (1024 + code, or 64 + code
-// from the field one place further up, less the rest, both exact).
+// Weights code - 8 of inputs 2 i and 2 i + 1 of a word of 8 codes as 16-bit floats: BF16 128 + code less 136, FP16 1024 + code (or 64 + code,
+// from the field one place further up) less the rest, all exact.
 template <bool PAIR>
 __device__ __forceinline__ uint32_t weights2(uint32_t word, int i) {
   if (PAIR) {
@@ -51,7 +51,9 @@ __device__ __forceinline__ uint32_t weights2(uint32_t word, int i) {
     const __half2 w = i & 1 ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hsub2(h, __float2half2_rn(1032.f));
     return *reinterpret_cast<const uint32_t*>(&w);
   }
-  return ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  const uint32_t u = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  const __nv_bfloat162 w = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(136.f));
+  return *reinterpret_cast<const uint32_t*>(&w);
 }
 
 // 16 inputs of one row: as they come, and as operand words (word 2 s + e: inputs 4 s + 2 e and 4 s + 2 e + 1).
@@ -135,7 +137,7 @@ struct Tokens {
 #pragma unroll
       for (int e = 0; e < 4; ++e) base[t][e] = 0.f;
       if constexpr (!PAIR) {
-        const uint32_t f[4] = {0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u};  // -136
+        const uint32_t f[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int s = 0; s < 4; ++s) mma16<PAIR>(base[t], f, x[t].w[0][2 * s], x[t].w[0][2 * s + 1], base[t]);
       }
@@ -299,8 +301,13 @@ struct Variant {
   }
 };
 // Few tiles of outputs for a CTA: 16 warps share the inputs' length, which is latency. Many: 8 warps, whose registers hold more tiles, so
-// that what is done once for 64 inputs serves more outputs. us with few / many, 8 rows: 2304 x 768 FP32 2.6 / 3.3, 6400 x 1600 BF16 3.8 / 4.8,
-// 28672 x 8192 BF16 40 / 38. (Weights through a ring of shared memory, bulk copies: as fast as these loads into registers, 37 to 39.)
+// that what is done once for 64 inputs serves more outputs. us with few / many (444 tiles are 7104 outputs on 148 SMs; weights through a ring of
+// shared memory, bulk copies, were as fast as these loads into registers):
+//                  rows:  1            8            16              rows:  1            8           16
+//   4096 x 4096    BF16 5.0 / 7.2    5.1 / 7.2    6.8 / 8.8      FP32 6.1 / 9.1    6.4 / 9.2   10.0 / 13.5
+//   6400 x 1600    BF16 3.7 / 4.5    3.9 / 4.7    5.2 / 5.7      FP32 5.6 / 5.6    6.3 / 6.0   10.0 / 8.3
+//   7600 x 2000    BF16 5.4 / 5.4    5.6 / 5.6    7.9 / 7.2      FP32 6.6 / 6.7    7.6 / 7.1   12.1 / 10.1
+//   16384 x 4096   BF16 14.1 / 12.9  14.5 / 13.2  19.4 / 16.7    FP32 19.3 / 15.9  22.1 / 16.4  35.6 / 23.1
 template <typename T, int NT>
 struct Choice {
   static constexpr bool PAIR = std::is_same<T, float>::value;

@@ -861,3 +861,22 @@ def test_attention_queries_at_the_ends_of_the_range(size, rows, dtype):
     out = torch.full_like(q, 1e4)
     cache.handle.attention(q, out, i32([300]), workspace(cache, rows, 2, dtype), row_start=starts([rows]), max_rows=rows, scale=0.125 / size)
     check_attention(cache, q, out, [rows], 0.125 / size)
+
+
+def test_linear_q4_outlier_with_weights_of_zero():
+    """An input that is far larger than the others of its row and meets weights of zero: the sums do not know it. Sums as in test_linear_q4."""
+    n, k = 48, 256
+    w = torch.randn(n, k, generator=gen(1), device=DEV)
+    w[:, 70] = 0
+    ps, ss = pg.q4_shapes(n, k, 64)
+    packed, scales = torch.empty(ps, dtype=torch.uint8, device=DEV), torch.empty(ss, dtype=BF16, device=DEV)
+    pg.quantize_q4(w, packed, scales, 64)
+    w = ref.q4_weights(packed, scales, n, k, 64)
+    assert (w[:, 70] == 0).all()
+    for m in (3, 16):
+        x = torch.randn(m, k, generator=gen(2), device=DEV).to(BF16)
+        x[:, 70] = torch.logspace(3, 8, m, device=DEV).to(BF16)
+        out = torch.empty(m, n, device=DEV, dtype=BF16)
+        pg.linear_q4(x, packed, scales, out, 64)
+        want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+        assert ((out.double() - want).abs() <= 2.0 ** -18 * size + U[BF16] * want.abs()).all()
