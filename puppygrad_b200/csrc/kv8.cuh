@@ -26,6 +26,10 @@ __device__ __forceinline__ int page_of(const Kv8View& c, int b, int lp) {
   return (unsigned)page < (unsigned)c.n_pages ? page : -1;
 }
 
+// Softmax weights go to FP16 as up to 2^15, its upper end: their rounding, 2^-25 below its normal numbers, is then 2^-40 of the largest, and a long tail
+// of small weights is not lost. Maxima are rounded up and what is taken from an exponent down, so that no weight is larger.
+constexpr float WEIGHT_BITS = 15.f;
+
 // Two e4m3 codes (low and high byte) as FP16, exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   uint32_t r;

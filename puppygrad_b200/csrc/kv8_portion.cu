@@ -7,20 +7,20 @@
 // so both are K-major as they come. Four softmax warps for each tile have a row for every thread, which needs no exchange between
 // threads; one warp issues the products, the scores of a piece in front of the values of the one before it, so that the tensor pipe
 // works while the softmax of the next scores is computed. Two tiles share the producers' work at head_dim 128 (1500 rows behind 2600
-// positions of two sequences, 32 query heads: 236 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are
-// better (1000 rows of four sequences, 12 heads: 41 us, 55 us), above 128 tensor memory has room for one.
+// positions of two sequences, 32 query heads: 237 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are
+// better (1000 rows of four sequences, 12 heads: 42 us, 55 us), above 128 tensor memory has room for one.
 // Where the tiles are too few for the chip, each is cut along the positions (grid y); the parts, FP32 with their maxima and sums, are
 // merged by a kernel of their own in the order of the positions.
 //
 // Scales, weights and the running maximum are those of the step kernel: the value scale is part of the exponent, the denominator
 // divides it out. The maximum that weights refer to (a whole number: less the blocks' exponents it is exact) moves only when a row
-// outgrows it by 2^8 (FP16 holds 2^15), which spares most passes over O. FP32 rows are pairs of FP16 numbers, queries and weights alike:
+// outgrows it by 2^3, which spares most passes over O; weights are up to 2^12 there, which leaves those to FP16's range. FP32 rows are pairs of FP16 numbers, queries and weights alike:
 // two products into the same accumulator.
 //
 // Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy at
 // head_dim 128, 1024 cycles for 256 rows and 64 positions. Measured there: 2700 cycles. A softmax warp takes 400 for the maximum, 250 to
-// get the scores, 1200 for exponentials, sums and stores, and two of them share a scheduler and its special functions; 0.6 PFLOP/s, 236 us
-// for the portions above, 403 us with FP32 rows. Three producer warps are too few at 128 (321 us), seven no better than four (249 us);
+// get the scores, 1200 for exponentials, sums and stores, and two of them share a scheduler and its special functions; 0.6 PFLOP/s, 237 us
+// for the portions above, 406 us with FP32 rows. Three producer warps are too few at 128 (321 us), seven no better than four (249 us);
 // above 128 eight are better than four (head_dim 256, 1000 rows of four sequences: 158 us, 168 us).
 #include <algorithm>
 #include <type_traits>
@@ -32,6 +32,9 @@ namespace pg {
 namespace {
 
 constexpr int ROWS = 128, TOKENS = 64, TILE_WARPS = 4;
+constexpr float LAG = 3.f, LIFT = WEIGHT_BITS - LAG;  // a row's weights are up to 2^LIFT where its maximum is up to date
+constexpr float LOWER = 0x1p-12f;                     // 2^-LIFT: denominators are without that factor, which keeps them in FP32's range
+static_assert(LIFT == 12.f, "LOWER");
 
 template <int DP, typename T>
 struct PortionShape {
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
   __shared__ uint64_t q_full[TILES], full[STAGES], empty[STAGES], s_full[TILES][2], p_full[TILES][2], o_done[TILES];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_flag;
-  __shared__ float4 info[STAGES][3];  // of a stage's four pieces of 16 tokens: key scale, log2 of the value scale, its inverse
+  __shared__ float4 info[STAGES][3];  // of a stage's four pieces of 16 tokens: key scale, log2 of the value scale, 2^-LIFT times its inverse
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* stages = base + S::QUERIES;
   volatile int* failed = &failed_flag;
@@ -304,9 +307,9 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         float m = fmaxf(v[h * 16], v[h * 16 + 1]);
 #pragma unroll
         for (int e = 2; e < 16; e += 2) m = fmaxf(m, fmaxf(v[h * 16 + e], v[h * 16 + e + 1]));
-        t_max = fmaxf(t_max, fmaf(m, kf[h], ev[h]));
+        t_max = fmaxf(t_max, __fmaf_ru(m, kf[h], ev[h]));
       }
-      if (__any_sync(ALL_LANES, t_max > m_ref + 8.f)) {
+      if (__any_sync(ALL_LANES, t_max > __fadd_rd(m_ref, LAG))) {
         const float m_new = fmaxf(m_ref, ceilf(t_max)), corr = m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new);
         m_ref = m_new;
         sum *= corr;
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const float b = ev[h] - m_use;
+        const float b = __fadd_rd(__fsub_rd(ev[h], m_use), LIFT);
         const unsigned long long k2 = pack2(kf[h], kf[h]), b2 = pack2(b, b);
         unsigned long long part = pack2(0.f, 0.f);
         uint32_t hi16[8], lo16[8];
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
           rows_out<float, DP / 2>(mine, tmem_o + d, any, fill, 1.f, DP / 2, true, [&](int k) { return row_w + k < rows ? to + (row_w + k) * DP + d : nullptr; });
       } else {
         const int64_t at = (int64_t)(r.first + tok) * a.out_row + entry;
-        rows_out<T, DP>(mine, tmem_o, any, fill, sum == 0.f ? 0.f : 1.f / sum, c.dim, wide_of(a.out, a.out_row), [&](int k) {
+        rows_out<T, DP>(mine, tmem_o, any, fill, sum == 0.f ? 0.f : LOWER / sum, c.dim, wide_of(a.out, a.out_row), [&](int k) {
           T* p = (T*)a.out + __shfl_sync(ALL_LANES, at, k);
           return row_w + k < rows ? p : nullptr;
         });
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         float* to = reinterpret_cast<float*>(&info[stage][0]) + p_tid;
         to[0] = page < 0 ? 1.f : scale.x;
         to[4] = page < 0 ? -INFINITY : odd ? scale.y : __log2f(sv);
-        to[8] = page < 0 || odd ? 1.f : 1.f / sv;
+        to[8] = page < 0 || odd ? 1.f : LOWER / sv;
       }
       fence_async_proxy();
       __syncwarp();
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(128) kv8_portion_merge_kernel(Kv8AttnArgs a, i
   // a lane for a part (at most 32): its maximum, what it is to be multiplied with
   const float2 ml = lane < w.parts ? *reinterpret_cast<const float2*>(from + lane * step + (size_t)(SIZE - i) * DP + 2 * i) : make_float2(-INFINITY, 0.f);
   const float top = lane_max(ml.x), f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - top), sum = lane_sum(ml.y * f);
-  const float by = sum == 0.f ? 0.f : 1.f / sum;
+  const float by = sum == 0.f ? 0.f : LOWER / sum;
   const int x = w.row0 + i, tok = x / a.group;
   T* out = (T*)a.out + (size_t)(w.r.first + tok) * a.out_row + (size_t)(head * a.group + (x - tok * a.group)) * c.dim;
   float o[DP / 32];

@@ -15,9 +15,9 @@
 //
 // Softmax with the blocks' scales: the key scale multiplies the score, the value scale is part of the exponent, w = 2^(s log2 e +
 // log2 scale_v - m), so that O = sum w code and the weights stay within [0, 1] however the scales differ; the denominator adds w /
-// scale_v. m is the running maximum of that exponent, rounded up. FP32 queries and their weights are pairs of FP16 numbers, two instructions
-// into one accumulator: FP32 grade. Rounding: BF16 queries are exact in FP16 after their row's scaling to [1, 2), their weights round
-// to FP16 (2^-12 of the largest).
+// scale_v. m is the running maximum of that exponent, rounded up, less 15: FP16 holds up to 2^16, and what rounds to nothing at its lower end
+// is then below 2^-40 of the largest. FP32 queries and their weights are pairs of FP16 numbers, two instructions into one accumulator: FP32
+// grade. Rounding: BF16 queries are exact in FP16 after their row's scaling to [1, 2), their weights round to FP16 (2^-11 of each).
 //
 // Bound: memory, at HBM's rate while bytes are on their way. Beside them a call takes the start (units counted, page table, scales: 4300
 // cycles until the first bytes are asked for), the SMs' different speeds (equal shares end 20% apart) and the merges (10000 cycles where
@@ -32,6 +32,7 @@ namespace pg {
 namespace {
 
 constexpr int UNIT = 64;  // positions
+constexpr float LOWER = 0x1p-15f;  // 2^-WEIGHT_BITS: denominators are without that factor, which keeps them in FP32's range
 
 // Bytes come through a ring of slots for every warp, 64 tokens times 64 head entries (4 KB) each, keys of a unit first, then its
 // values: all but one are on their way while that one is worked on, 128 KB for an SM.
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
         // ---- exponents; masked ones are -infinity whatever the bytes were
         const float sv = fmaxf(cur.scale.y, 7.888609e-31f);  // 2^-100, the least scale that an append writes
         const bool odd = cur.scale.y != cur.scale.y;
-        const float ev = odd ? cur.scale.y : __log2f(sv), inv_v = odd ? 1.f : 1.f / sv;
+        const float ev = odd ? cur.scale.y : __log2f(sv), inv_v = odd ? 1.f : LOWER / sv;
         const bool whole = __all_sync(ALL_LANES, cur.page >= 0) && t0 + UNIT - 1 <= pos_low && t0 + UNIT <= t.have &&
                            (a.window == 0 || t0 > pos_high - a.window || t0 + UNIT <= a.keep);
         uint32_t ph[NB][8], pl[PAIR ? NB : 1][8];
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
             raw[0] = fmaxf(raw[0], fmaxf(s[j][n][0], s[j][n][2]));
             raw[1] = fmaxf(raw[1], fmaxf(s[j][n][1], s[j][n][3]));
           }
-          float top[2] = {fmaxf(m[n][0], ceilf(fmaf(raw[0], f0, add))), fmaxf(m[n][1], ceilf(fmaf(raw[1], f1, add)))};
+          float top[2] = {fmaxf(m[n][0], ceilf(__fmaf_ru(raw[0], f0, add))), fmaxf(m[n][1], ceilf(__fmaf_ru(raw[1], f1, add)))};
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
             top[0] = fmaxf(top[0], __shfl_xor_sync(ALL_LANES, top[0], off));
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
             const float base = top[e] == -INFINITY ? 0.f : top[e];
             down[n][e] = ex2(m[n][e] - base);
             m[n][e] = top[e];
-            top[e] = add - base;
+            top[e] = __fadd_rd(__fsub_rd(add, base), WEIGHT_BITS);
           }
           float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
             const int row = n * 8 + cc * 2 + e, x = t.row0 + row, r = t.n_rows == 1 ? 0 : x / a.group;
             if (row >= t.rows) continue;
             T* to = (T*)a.out + (size_t)(t.first_row + r) * a.out_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim;
-            const float f = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+            const float f = l[n][e] == 0.f ? 0.f : LOWER / l[n][e];
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
               if (16 * i + g < c.dim) to[16 * i + g] = from_f32<T>(o[i][n][e] * f);
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
   auto put = [&](const Tile& t, int i, int d, const float4& v, float l) {
     const int x = t.row0 + i, r = t.n_rows == 1 ? 0 : x / a.group;
     T* to = (T*)a.out + (size_t)(t.first_row + r) * a.out_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim + d;
-    const float f = l == 0.f ? 0.f : 1.f / l;
+    const float f = l == 0.f ? 0.f : LOWER / l;
     const float w[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
 #pragma unroll
     for (int e = 0; e < 4; ++e)

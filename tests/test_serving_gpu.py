@@ -880,3 +880,29 @@ def test_linear_q4_outlier_with_weights_of_zero():
         pg.linear_q4(x, packed, scales, out, 64)
         want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
         assert ((out.double() - want).abs() <= 2.0 ** -18 * size + U[BF16] * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("seqs,rows,heads,dim", [(2400, 1, 1, 64), (100, 2, 128, 64), (80, 2, 128, 128)])  # few rows of a sequence, portions; tiles that are not cut
+def test_attention_long_tail_behind_one_large_weight(seqs, rows, heads, dim, dtype):
+    """One token outweighs each of the 131071 others by 2^25.6, and they together are 2.6 thousandths: the mean of their equal values must keep them."""
+    n, page = 131072, 64
+    pages = n // page
+    pool = torch.zeros(pg.Kv8Cache.pool_shape(pages, 1, page, dim), dtype=torch.uint8, device=DEV)
+    keys, values = ref.blocks(pool, page, dim)
+    keys[0, 0, 0, 0] = 0x38  # 1: the first token's score is 17.75, the others' 0
+    values[..., :dim, :] = 0x38
+    values[0, 0, :, 0] = 0
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).repeat(seqs, 1)  # sequences may share pages
+    cache = pg.Kv8Cache(pool, torch.ones(pages, 1, 2, device=DEV), table, page_tokens=page, head_dim=dim)
+    q = torch.zeros(seqs * rows, heads, dim, device=DEV, dtype=dtype)
+    q[..., 0] = 17.75
+    out = torch.full_like(q, 7.0)
+    ws = torch.zeros(cache.workspace_bytes(seqs * rows, heads, dtype), dtype=torch.uint8, device=DEV)
+    cache.attention(q, out, i32([n] * seqs), ws, row_start=starts([rows] * seqs), max_rows=rows, scale=1.0)
+    for r in range(rows):
+        tail = (n - rows + r) * math.exp(-17.75)
+        want = tail / (1 + tail)
+        # weights to half a step each (FP32 rows: pairs and their sums, 2^-15 of the result; BF16: FP16 numbers), tokens not lost but rounded to 2^-37 of the largest
+        tol = want * (2.0 ** -15 if dtype == F32 else 2.0 ** -10 + 2.0 ** -8) + n * 2.0 ** -37
+        assert ((out[r::rows].double() - want).abs() <= tol).all(), (float(out[r::rows].double().min()), want)
