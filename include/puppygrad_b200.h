@@ -386,7 +386,8 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
  * as in pg_kv8_append, whose `lens` it takes; query head h reads key / value head h / (heads / kv_heads). A row that sees nothing
  * gets zeros; rows outside row_start[0]..row_start[seqs]-1 are left as they were. max_rows: at least the rows of any sequence
  * (it chooses the kernels; a sequence with more is still computed). Where row_start decreases, rows are left out or computed twice. FP32 queries are computed to FP32 grade from pairs of
- * FP16 numbers, BF16 queries with FP16 probabilities; sums are FP32. Entries of q times scale, and scores, have to stay below 2^120: a row
+ * FP16 numbers, BF16 queries with FP16 probabilities; sums are FP32 (many rows of a sequence: the matrix unit's, which cut off; within
+ * 10^-5 for FP32 queries, 4 * 10^-9 for every position for BF16 ones). Entries of q times scale, and scores, have to stay below 2^120: a row
  * beyond that may be NaN.
  * workspace: pg_kv8_attention_workspace_bytes() bytes, 256-byte aligned, zeroed by the caller before its first use and left ready for the next
  * call, whatever that one's cache, rows, heads and type are, as long as the workspace has the bytes it needs. Calls that may overlap on the

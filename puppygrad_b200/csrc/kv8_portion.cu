@@ -9,6 +9,10 @@
 // works while the softmax of the next scores is computed. Two tiles share the producers' work at head_dim 128 (1500 rows behind 2600
 // positions of two sequences, 32 query heads: 237 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are
 // better (1000 rows of four sequences, 12 heads: 42 us, 55 us), above 128 tensor memory has room for one.
+// The instruction cuts off what it adds to O, up to 5*10^-8 of it each time, and always towards zero, so that sums of one sign drift: 4*10^-4 over 65536
+// positions of FP32 rows. Theirs therefore join sums in memory (a place of the workspace for each CTA that is running) after every 32 pieces, by rounded
+// additions, and O starts anew: within 10^-5 for 11% of the time (16 pieces: 3*10^-6, 14%). BF16 rows, with half as many
+// products, drift by less than their result's rounding up to 10^6 positions and are left.
 // Where the tiles are too few for the chip, each is cut along the positions (grid y); the parts, FP32 with their maxima and sums, are
 // merged by a kernel of their own in the order of the positions.
 //
@@ -20,7 +24,7 @@
 // Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy at
 // head_dim 128, 1024 cycles for 256 rows and 64 positions. Measured there: 2700 cycles. A softmax warp takes 400 for the maximum, 250 to
 // get the scores, 1200 for exponentials, sums and stores, and two of them share a scheduler and its special functions; 0.6 PFLOP/s, 237 us
-// for the portions above, 406 us with FP32 rows. Three producer warps are too few at 128 (321 us), seven no better than four (249 us);
+// for the portions above, 452 us with FP32 rows. Three producer warps are too few at 128 (321 us), seven no better than four (249 us);
 // above 128 eight are better than four (head_dim 256, 1000 rows of four sequences: 158 us, 168 us).
 #include <algorithm>
 #include <type_traits>
@@ -45,7 +49,10 @@ struct PortionShape {
   static constexpr int TILE_QUERIES = (PAIR ? 2 : 1) * KC * 16384, QUERIES = TILES * TILE_QUERIES, HALF = KC * 8192, STAGE = 2 * HALF;  // bytes
   static constexpr int STAGES = QUERIES + 3 * STAGE <= (DP == 64 ? 100 : 192) * 1024 ? 3 : QUERIES + 2 * STAGE <= 192 * 1024 ? 2 : 1;
   static constexpr int SMEM = QUERIES + STAGES * STAGE + 1024;
-  static constexpr int CTAS = DP == 64 ? 2 : 1;  // for an SM
+  static constexpr int CTAS = DP == 64 ? 2 : 1;       // for an SM
+  static constexpr int KEEP = 32;                     // pieces after which the sums of FP32 rows join those in memory
+  static constexpr int PLACES = KV8_MAX_CTAS * CTAS;  // for those
+  static_assert(TILES * ROWS * CTAS * (DP + 1) == kv8_held(DP) && PLACES <= KV8_PLACES, "the workspace");
   static constexpr int COLS = 512 / CTAS;  // tensor memory: for each tile O, then two places for scores and weights
   static_assert(TILES * (DP + 128) <= COLS, "tensor memory");
 };
@@ -89,9 +96,10 @@ __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.
 
 // A warp's 32 rows of COLS sums out of tensor memory, times a factor for each, to rows of `dim` entries at to(row) (null: none). A thread has
 // a row there, and neighbouring threads get neighbouring 16 bytes of one here: through shared memory (32 * COLS * sizeof(E) bytes). Where
-// there are no sums (any = false) the rows get `fill`, and that memory, which may still be in use, is left alone.
+// there are no sums (any = false) the rows get `fill`, and that memory, which may still be in use, is left alone. `held` (or null): more sums of this thread's
+// row, a column every `step`, to be multiplied with f.
 template <typename E, int COLS, typename F>
-__device__ __forceinline__ void rows_out(uint8_t* mine, uint32_t taddr, bool any, float fill, float by, int dim, bool wide, F to) {
+__device__ __forceinline__ void rows_out(uint8_t* mine, uint32_t taddr, bool any, float fill, const float* held, int step, float f, float by, int dim, bool wide, F to) {
   constexpr int PER = 16 / sizeof(E), VECS = COLS / PER;
   static_assert(VECS % 8 == 0, "places are swapped among eight");
   const int lane = threadIdx.x & 31;
@@ -99,6 +107,10 @@ __device__ __forceinline__ void rows_out(uint8_t* mine, uint32_t taddr, bool any
   for (int d = 0; d < COLS && any; d += 16) {
     float o[16];
     tmem_ld16(taddr + d, o);
+    if (held) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = fmaf(__ldcg(held + (d + e) * step), f, o[e]);
+    }
     union {
       uint4 u[16 / PER];
       E t[16];
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t q_full[TILES], full[STAGES], empty[STAGES], s_full[TILES][2], p_full[TILES][2], o_done[TILES];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed_flag;
+  __shared__ int failed_flag, place;  // place: of this CTA's sums in memory
   __shared__ float4 info[STAGES][3];  // of a stage's four pieces of 16 tokens: key scale, log2 of the value scale, 2^-LIFT times its inverse
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* stages = base + S::QUERIES;
@@ -210,6 +222,13 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
       mbar_init(&o_done[i], 1);
     }
     failed_flag = 0;
+    place = -1;
+    if (PAIR && pieces > S::KEEP) {
+      // there are as many places as CTAs can run at once, so one is free
+      for (int i = 0, p = blockIdx.x % S::PLACES; i < S::PLACES && place < 0; ++i, p = p + 1 == S::PLACES ? 0 : p + 1)
+        if (atomicCAS(a.places + p, 0u, 1u) == 0u) place = p;
+      __threadfence();
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == SOFTMAX_WARPS) tmem_alloc(&tmem_slot, S::COLS);
@@ -218,7 +237,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   auto o_of = [&](int t) { return tmem + (uint32_t)(t * (DP + 128)); };
-  bool ok = true;
+  bool ok = !PAIR || place >= 0 || pieces <= S::KEEP;
 
   if (warp < SOFTMAX_WARPS) {
     // ---- a row for every thread
@@ -278,6 +297,13 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
     }
 
     float m_ref = -INFINITY, sum = 0.f;
+    // sums in memory, then the maximum that they refer to: [column][row], so that lanes are neighbours
+    constexpr int NEXT = TILES * ROWS;
+    auto held_at = [&] { return a.held + (size_t)max(place, 0) * (DP + 1) * NEXT + tile * ROWS + in_tile; };
+    auto held_factor = [&](const float* held) {
+      const float m = __ldcg(held + DP * NEXT);
+      return m == -INFINITY ? 0.f : ex2(m - m_ref);
+    };
     int stage = 0;
     for (int j = 0; j < pieces && used; ++j) {
       const uint32_t s_at = tmem_s + (uint32_t)(j & 1) * 64;
@@ -358,6 +384,21 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
       // each product is waited for before the next one can be issued: a wait by parity knows two phases apart no more (by now it is done)
       if (j > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (j - 1) & 1, failed, nullptr, 0));
       if (!ok) break;
+      if (PAIR && j > 0 && j % S::KEEP == 0) {
+        tc_fence_after();
+        float* held = held_at();
+        const float f = j == S::KEEP ? 0.f : held_factor(held);
+#pragma unroll 1
+        for (int d = 0; d < DP; d += 16) {
+          float o[16], h[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) h[e] = j == S::KEEP ? 0.f : __ldcg(held + (d + e) * NEXT);
+          tmem_ld16(tmem_o + d, o);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) __stcg(held + (d + e) * NEXT, fmaf(h[e], f, o[e]));
+        }
+        __stcg(held + DP * NEXT, m_ref);
+      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -371,15 +412,17 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
       uint8_t* mine = base + tile * S::TILE_QUERIES + (warp & 3) * (S::TILE_QUERIES / 4);  // the queries are not needed any more
       const int row_w = tile * ROWS + (warp & 3) * 32;  // the warp's first row
       const bool any = pieces > 0 && ok;
+      const float* more = PAIR && pieces > S::KEEP && ok ? held_at() : nullptr;
+      const float f = more ? held_factor(more) : 0.f;
       if (w.parts > 1) {
         float* to = a.partials + ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * (TILES * ROWS) * (DP + 2);
         if (i < rows) *reinterpret_cast<float2*>(to + (size_t)TILES * ROWS * DP + 2 * i) = make_float2(m_ref, sum);
 #pragma unroll 1
         for (int d = 0; d < DP; d += DP / 2)
-          rows_out<float, DP / 2>(mine, tmem_o + d, any, fill, 1.f, DP / 2, true, [&](int k) { return row_w + k < rows ? to + (row_w + k) * DP + d : nullptr; });
+          rows_out<float, DP / 2>(mine, tmem_o + d, any, fill, more ? more + d * NEXT : nullptr, NEXT, f, 1.f, DP / 2, true, [&](int k) { return row_w + k < rows ? to + (row_w + k) * DP + d : nullptr; });
       } else {
         const int64_t at = (int64_t)(r.first + tok) * a.out_row + entry;
-        rows_out<T, DP>(mine, tmem_o, any, fill, sum == 0.f ? 0.f : LOWER / sum, c.dim, wide_of(a.out, a.out_row), [&](int k) {
+        rows_out<T, DP>(mine, tmem_o, any, fill, more, NEXT, f, sum == 0.f ? 0.f : LOWER / sum, c.dim, wide_of(a.out, a.out_row), [&](int k) {
           T* p = (T*)a.out + __shfl_sync(ALL_LANES, at, k);
           return row_w + k < rows ? p : nullptr;
         });
@@ -433,7 +476,7 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
             for (int p = PAIR ? 1 : 0; p >= 0; --p)
 #pragma unroll
               for (int k = 0; k < TOKENS / 16; ++k)
-                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, j != 0 || p != (PAIR ? 1 : 0) || k != 0);
+                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (PAIR ? j % S::KEEP : j) != 0 || p != (PAIR ? 1 : 0) || k != 0);
             umma_commit(&o_done[t]);
             if (t == tiles - 1) umma_commit(&empty[now.stage]);
           }
@@ -535,6 +578,10 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
   __syncthreads();
   tc_fence_after();
   if (warp == SOFTMAX_WARPS) tmem_dealloc(tmem, S::COLS);
+  if (PAIR && tid == 0 && place >= 0) {
+    __threadfence();
+    atomicExch(a.places + place, 0u);
+  }
 }
 
 // Puts the parts of a row together: a warp for a row.

@@ -108,11 +108,15 @@ Kv8View view(const pg_kv8_cache* c) {
           c->kv_heads, c->head_dim, c->seqs, c->pages_per_seq};
 }
 
-// A workspace: counters of the step kernel, one for each of its CTAs, then parts of tiles: two for every CTA and one for each of its warps, of
-// which there are 16 with tiles of 8 rows, 8 with tiles of 16. Where the counters lie is the same for all calls: parts that one call
-// leaves are never what the next one counts with.
-constexpr size_t COUNTER_BYTES = 1024;
-static_assert(COUNTER_BYTES >= KV8_MAX_CTAS * 4, "a counter for each CTA");
+// A workspace: counters of the step kernel, one for each of its CTAs, and which of the portion kernel's places are taken; for FP32 rows the sums in
+// those places; then parts of tiles: two for every CTA of the step kernel and one for each of its warps, of which there are 16 with tiles of 8
+// rows, 8 with tiles of 16. Where the words lie that have to be zero between calls is the same for all calls: parts that one leaves are
+// never what the next one counts with.
+constexpr size_t PLACES_AT = 1024, SUMS_AT = 4096;
+static_assert(PLACES_AT >= KV8_MAX_CTAS * 4 && SUMS_AT >= PLACES_AT + KV8_PLACES * 4, "a counter for each CTA, a word for each place");
+size_t held_bytes(const pg_kv8_cache* c, int dtype) {
+  return dtype == PG_DTYPE_F32 ? ((size_t)KV8_MAX_CTAS * kv8_held(kv8_padded(c->head_dim)) * 4 + 255) / 256 * 256 : 0;
+}
 size_t partial_bytes(const pg_kv8_cache* c) {
   const int padded = kv8_padded(c->head_dim), rows = padded == 64 ? (2 + 16) * 16 : std::max((2 + 16) * 8, (2 + 8) * 16);
   // (the portion kernel, which runs behind the step kernel, cuts its tiles of 128 or 256 rows into as many parts)
@@ -162,7 +166,7 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
 uint64_t pg_kv8_attention_workspace_bytes(const pg_kv8_cache* cache, int32_t rows, int32_t heads, int32_t dtype) {
   if (check_cache(cache) || check_dtype(dtype) || check_heads(cache, heads)) return 0;
   if (rows < 0) return bad("rows must not be negative"), 0;
-  return COUNTER_BYTES + partial_bytes(cache);
+  return SUMS_AT + held_bytes(cache, dtype) + partial_bytes(cache);
 }
 
 int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, void* out, int64_t out_row, int32_t dtype,
@@ -193,8 +197,10 @@ int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, vo
   if (window > INT32_MAX / 2) window = 0;  // wider than any table: its arithmetic stays within 32 bits
   // rows that fill less than half a tile of the portion kernel, and all of them where it has no table of rows
   const bool portions = row_start && (int64_t)group * max_rows > KV8_STEP_ROWS;
+  char* const sums = (char*)workspace + SUMS_AT;
   Kv8AttnArgs a{view(cache), q, out, q_row, out_row, heads, group, rows, max_rows, row_start, lens, scale, window, window > 0 ? keep_first : 0,
-                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)workspace, (float*)((char*)workspace + COUNTER_BYTES)};
+                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)workspace, (unsigned*)((char*)workspace + PLACES_AT),
+                (float*)(sums + held_bytes(cache, dtype)), (float*)sums};
   if (!portions) return launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention");
   a.max_rows = std::min(max_rows, (KV8_STEP_ROWS + group - 1) / group);
   if (int r = launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention")) return r;

@@ -14,8 +14,11 @@ constexpr int KV8_MAX_SEQS = 4096;
 // 269 / 290, 387 / 302, 513 / 312; 12 heads of 64 BF16 137 / 180, 176 / 185, 241 / 201; 8 of 4000, 4 heads of 256, BF16 64 / 59, 88 / 69, 106 / 70.
 constexpr int KV8_STEP_ROWS = 40;
 constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace does not hang on the device
+constexpr int KV8_PLACES = 2 * KV8_MAX_CTAS;  // for sums in memory of CTAs of the portion kernel, of which two run on an SM at head_dim 64
 
 __host__ __device__ inline int kv8_padded(int head_dim) { return (head_dim + 63) / 64 * 64; }
+// Floats of those sums for an SM: of 256 rows (128 above head_dim 128), with a maximum for each.
+__host__ __device__ constexpr int kv8_held(int padded) { return (padded <= 128 ? 256 : 128) * (padded + 1); }
 
 // The cache as the kernels see it.
 struct Kv8View {
@@ -44,8 +47,8 @@ struct Kv8AttnArgs {
   float scale;
   int window, keep;
   int step_rows;  // sequences of at most so many (token, head of the group) rows are the step kernel's, the others the portion kernel's
-  unsigned* counters;
-  float* partials;
+  unsigned *counters, *places;
+  float *partials, *held;
 };
 struct Q4Args {
   const void *x, *bias;

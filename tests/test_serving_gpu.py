@@ -906,3 +906,30 @@ def test_attention_long_tail_behind_one_large_weight(seqs, rows, heads, dim, dty
         # weights to half a step each (FP32 rows: pairs and their sums, 2^-15 of the result; BF16: FP16 numbers), tokens not lost but rounded to 2^-37 of the largest
         tol = want * (2.0 ** -15 if dtype == F32 else 2.0 ** -10 + 2.0 ** -8) + n * 2.0 ** -37
         assert ((out[r::rows].double() - want).abs() <= tol).all(), (float(out[r::rows].double().min()), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("seqs,rows,heads", [(2400, 1, 1), (40, 3, 128), (1, 130, 2)])  # few rows of a sequence; portions in one part, in several
+def test_attention_long_sums_of_values_of_one_sign(seqs, rows, heads, dim, dtype):
+    """Values around 1: the sums over 40000 tokens only grow, and whatever cuts them off adds up."""
+    n, page = 40000, 64
+    pages, g = -(-n // page), gen(dim)
+    pool = torch.zeros(pg.Kv8Cache.pool_shape(pages, 1, page, dim), dtype=torch.uint8, device=DEV)
+    keys, values = ref.blocks(pool, page, dim)
+    keys[..., :dim] = torch.randn(pages, 1, page, dim, generator=g, device=DEV).to(torch.float8_e4m3fn).view(torch.uint8)
+    values[..., :dim, :] = (1 + 0.25 * torch.randn(pages, 1, dim, page, generator=g, device=DEV)).to(torch.float8_e4m3fn).view(torch.uint8)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).repeat(seqs, 1)  # sequences may share pages
+    cache = pg.Kv8Cache(pool, torch.ones(pages, 1, 2, device=DEV), table, page_tokens=page, head_dim=dim)
+    q = torch.randn(seqs * rows, heads, dim, generator=g, device=DEV).to(dtype)
+    out = torch.full_like(q, 7.0)
+    ws = torch.zeros(cache.workspace_bytes(seqs * rows, heads, dtype), dtype=torch.uint8, device=DEV)
+    for call in range(2):
+        cache.attention(q, out, i32([n] * seqs), ws, row_start=starts([rows] * seqs), max_rows=rows)
+    k, v = ref.sequence_kv(pool, cache.scales, table[0], n, page, dim)
+    top, h = float(v.abs().max()), min(heads, 2)
+    for b in {0, seqs // 2, seqs - 1}:
+        some = slice(b * rows, b * rows + min(rows, 3))
+        want = ref.attention(q[some, :h].double(), k, v, torch.arange(n - rows, n, device=DEV)[:3], dim ** -0.5)
+        tol = top * (2.0 ** -15 if dtype == F32 else 2.0 ** -10) + U[dtype] * want.abs()
+        assert ((out[some, :h].double() - want).abs() <= tol).all(), (b, float(((out[some, :h].double() - want) / want).mean()))
