@@ -28,6 +28,13 @@ def _bad(what: str):
     return Gpt2Error("InvalidInput", what)
 
 
+def _checked(**numbers: int) -> None:
+    """The library takes these as 32 bits and would not see what is beyond. (Calls of a step "or" the numbers together first, which is quicker.)"""
+    for name, n in numbers.items():
+        if n >> 31:
+            raise _bad(f"{name} {n} must be in 0..2^31-1")
+
+
 def _code(t, name: str) -> int:
     code = _CODES.get(_name(t.dtype))
     if code is None:
@@ -84,7 +91,8 @@ class Kv8Cache:
 
     def __init__(self, pool, scales, page_table, page_tokens: int, head_dim: int):
         device = _device(pool, "pool")
-        _sides(page_table, "page_table", 2)
+        seqs, per_seq = _sides(page_table, "page_table", 2)
+        _checked(seqs=seqs, pages_per_seq=per_seq)
         n_pages, kv_heads = _sides(pool, "pool", 3)[:2]
         self._c = N.PgKv8Cache()
         self._c.pool = _flat(pool, "pool", "torch.uint8", self.pool_shape(n_pages, kv_heads, page_tokens, head_dim), device)
@@ -98,6 +106,7 @@ class Kv8Cache:
 
     @staticmethod
     def pool_shape(n_pages: int, kv_heads: int, page_tokens: int, head_dim: int) -> Tuple[int, int, int]:
+        _checked(n_pages=n_pages, kv_heads=kv_heads, page_tokens=page_tokens, head_dim=head_dim)
         size = N.lib.pg_kv8_pool_bytes(n_pages, page_tokens, kv_heads, head_dim)
         if not size:
             raise _bad(N.lib.pg_last_error_message().decode())
@@ -119,6 +128,8 @@ class Kv8Cache:
             shape = (rows, heads, self.head_dim)
             qp, qs = _rows(q, "q", kind, shape, device)
             op, os = _rows(q_out, "q_out", kind, shape, device)
+        if (rows | heads | rot_dims) >> 31:
+            _checked(rows=rows, heads=heads, rot_dims=rot_dims)
         lp = _flat(lens, "lens", "torch.int32", (self.seqs,), device)
         sp = 0 if row_start is None else _flat(row_start, "row_start", "torch.int32", (self.seqs + 1,), device)
         status = N.lib.pg_kv8_append(self._ref, kp, ks, vp, vs, qp, qs, op, os, dtype, heads, rows, sp, lp, rot_dims, rot_base, stream)
@@ -128,6 +139,7 @@ class Kv8Cache:
     def workspace_bytes(self, rows: int, heads: int, dtype) -> int:
         """Size of the workspace of `attention` calls of up to that many rows; its memory must be zero before its first use. Calls over
         different caches, rows and heads can share one, one after the other, if it has the most bytes that any of them needs."""
+        _checked(rows=rows, heads=heads)
         code = _CODES.get(_name(dtype), -1)
         size = N.lib.pg_kv8_attention_workspace_bytes(self._ref, rows, heads, code)
         if not size:
@@ -141,6 +153,8 @@ class Kv8Cache:
         before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each."""
         device, kind, shape = self.device, q.dtype, (*_sides(q, "q", 3)[:2], self.head_dim)
         rows, heads = shape[:2]
+        if (rows | heads | max_rows | window | keep_first) >> 31:
+            _checked(rows=rows, heads=heads, max_rows=max_rows, window=window, keep_first=keep_first)
         dtype = _code(q, "q")
         qp, qs = _rows(q, "q", kind, shape, device)
         op, os = _rows(out, "out", kind, shape, device)
@@ -156,6 +170,7 @@ class Kv8Cache:
 
 def q4_shapes(n: int, k: int, group: int) -> Tuple[Tuple[int, int, int], Tuple[int, int]]:
     """Shapes of the packed codes (uint8) and the scales (bfloat16) of a 4-bit matrix of n outputs and k inputs."""
+    _checked(n=n, k=k, group=group)
     if not N.lib.pg_q4_scale_bytes(n, k, group):
         raise _bad(N.lib.pg_last_error_message().decode())
     return (-(-n // 16), -(-k // 64), 512), (-(-k // group), -(-n // 16) * 16)
@@ -175,6 +190,8 @@ def linear_q4(x, packed, scales, out, group: int, bias=None, stream: int = 0) ->
     """out [m, n] = x [m, k] @ dequant(w [n, k]).T + bias for up to 16 rows."""
     m, k = _sides(x, "x", 2)
     n, kind = _sides(out, "out", 2)[1], x.dtype
+    if (m | n | k | group) >> 31:
+        _checked(m=m, n=n, k=k, group=group)
     dtype, device = _code(x, "x"), _device(x, "x")
     xp, xs = _rows(x, "x", kind, (m, k), device)
     op, os = _rows(out, "out", kind, (m, n), device)
@@ -191,6 +208,8 @@ def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=No
     """Scores of the rows of logits [rows, vocab]: logprobs [rows] of `targets` [rows], entropy [rows], the most likely ids and their
     log probabilities [rows, k] (k up to 32), each where its output is given."""
     rows, vocab = _sides(logits, "logits", 2)
+    if (rows | vocab) >> 31:
+        _checked(rows=rows, vocab=vocab)
     dtype, device, each = _code(logits, "logits"), _device(logits, "logits"), (rows,)
     lp, ls = _rows(logits, "logits", logits.dtype, (rows, vocab), device)
     if (top_ids is None) != (top_logprobs is None):
@@ -201,6 +220,7 @@ def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_ids=No
     k = ip = vp = 0
     if top_ids is not None:
         k = _sides(top_ids, "top_ids", 2)[1]
+        _checked(top_k=k)
         ip = _flat(top_ids, "top_ids", "torch.int32", (rows, k), device)
         vp = _flat(top_logprobs, "top_logprobs", "torch.float32", (rows, k), device)
     status = N.lib.pg_token_logprobs(lp, ls, dtype, rows, vocab, tp, op, ep, k, ip, vp, device, stream)

@@ -128,3 +128,45 @@ def test_buffers_with_another_number_of_dimensions_are_refused():
     for call in (lambda: pg.token_logprobs(x), lambda: pg.linear_q4(x, y, y, y, 64), lambda: pg.linear_q4(y, y, y, x, 64), lambda: pg.quantize_q4(x, y, y, 64)):
         with pytest.raises(pg.Gpt2Error, match=r"\(5,\) must have 2 dimensions"):
             call()
+
+
+class Buffer:
+    """What the operators look at of a tensor on a device; its address is never used by a call that is refused."""
+
+    def __init__(self, *shape, dtype=torch.float32):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, "cuda:0"
+
+    def stride(self):
+        return tuple(torch.empty(self.shape, device="meta").stride())
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return P
+
+
+def int32(*shape):
+    return Buffer(*shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("far", [1 << 31, (1 << 32) + 1, -1])
+def test_numbers_beyond_32_bits_are_refused(far):
+    """They would be taken modulo 2^32: a window of 2^32 for none at all, 2^32 rows for no rows."""
+    handle = pg.Kv8Cache(Buffer(4, 2, 2 * 16 * 64, dtype=torch.uint8), Buffer(4, 2, 2), int32(3, 5), page_tokens=16, head_dim=64)
+    q, k, lens, ws = Buffer(3, 4, 64), Buffer(3, 2, 64), int32(3), Buffer(1 << 30, dtype=torch.uint8)
+    calls = [lambda: handle.attention(q, q, lens, ws, window=far), lambda: handle.attention(q, q, lens, ws, keep_first=far),
+             lambda: handle.attention(q, q, lens, ws, row_start=int32(4), max_rows=far), lambda: handle.append(k, k, lens, rot_dims=far),
+             lambda: handle.workspace_bytes(far, 4, torch.float32), lambda: handle.workspace_bytes(3, far, torch.float32),
+             lambda: pg.q4_shapes(far, 64, 64), lambda: pg.q4_shapes(64, far, 64), lambda: pg.q4_shapes(64, 64, far), lambda: pg.Kv8Cache.pool_shape(far, 2, 16, 64),
+             lambda: pg.Kv8Cache.pool_shape(4, 2, 16, far), lambda: pg.linear_q4(Buffer(1, 64), Buffer(1, 1, 512, dtype=torch.uint8), Buffer(1, 16, dtype=torch.bfloat16), Buffer(1, 16), far)]
+    if far > 0:
+        calls += [lambda: pg.token_logprobs(Buffer(far, 1), entropy=Buffer(far)), lambda: pg.token_logprobs(Buffer(1, far), entropy=Buffer(1)),
+                  lambda: pg.token_logprobs(Buffer(1, 100), top_ids=int32(1, far), top_logprobs=Buffer(1, far)), lambda: handle.append(Buffer(far, 2, 64), Buffer(far, 2, 64), lens, row_start=int32(4)),
+                  lambda: pg.Kv8Cache(Buffer(4, 2, 2 * 16 * 64, dtype=torch.uint8), Buffer(4, 2, 2), int32(1, far), page_tokens=16, head_dim=64)]
+    for call in calls:
+        with pytest.raises(pg.Gpt2Error, match=f"{far} must be in 0..2\\^31-1"):
+            call()
