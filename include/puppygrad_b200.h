@@ -391,7 +391,8 @@ int pg_kv8_append(const pg_kv8_cache* cache, const void* k, int64_t k_row, const
  * beyond that may be NaN.
  * workspace: pg_kv8_attention_workspace_bytes() bytes, 256-byte aligned, zeroed by the caller before its first use and left ready for the next
  * call, whatever that one's cache, rows, heads and type are, as long as the workspace has the bytes it needs. Calls that may overlap on the
- * GPU (captured graphs among them) need workspaces of their own. */
+ * GPU (captured graphs among them) need workspaces of their own. Its first 32 bits become 1 where a bounded wait within a kernel ran out, whose rows
+ * are NaN then; no call sets them back. */
 uint64_t pg_kv8_attention_workspace_bytes(const pg_kv8_cache* cache, int32_t rows, int32_t heads, int32_t dtype);
 int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, void* out, int64_t out_row, int32_t dtype,
                      int32_t heads, int32_t rows, int32_t max_rows, const int32_t* row_start, const int32_t* lens, float scale,

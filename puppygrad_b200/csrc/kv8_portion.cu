@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
     if (ok && used && pieces > 0) ok = __all_sync(ALL_LANES, mbar_wait(&o_done[tile], (pieces - 1) & 1, failed, nullptr, 0));
     if (used) {
       tc_fence_after();
-      const float fill = ok ? 0.f : __uint_as_float(0x7FC00000u);  // a wait ran out: no result, and one that shows
+      const float fill = ok ? 0.f : __uint_as_float(0x7FC00000u);  // a wait ran out: no result, one that shows, and a word that says so
+      if (!ok && lane == 0) atomicExch(a.status, 1u);
       sum += fill;
       uint8_t* mine = base + tile * S::TILE_QUERIES + (warp & 3) * (S::TILE_QUERIES / 4);  // the queries are not needed any more
       const int row_w = tile * ROWS + (warp & 3) * 32;  // the warp's first row

@@ -108,12 +108,12 @@ Kv8View view(const pg_kv8_cache* c) {
           c->kv_heads, c->head_dim, c->seqs, c->pages_per_seq};
 }
 
-// A workspace: counters of the step kernel, one for each of its CTAs, and which of the portion kernel's places are taken; for FP32 rows the sums in
-// those places; then parts of tiles: two for every CTA of the step kernel and one for each of its warps, of which there are 16 with tiles of 8
+// A workspace: a word that says whether a wait ran out, counters of the step kernel, one for each of its CTAs, and which of the portion
+// kernel's places are taken; for FP32 rows the sums in those places; then parts of tiles: two for every CTA of the step kernel and one for each of its warps, of which there are 16 with tiles of 8
 // rows, 8 with tiles of 16. Where the words lie that have to be zero between calls is the same for all calls: parts that one leaves are
 // never what the next one counts with.
-constexpr size_t PLACES_AT = 1024, SUMS_AT = 4096;
-static_assert(PLACES_AT >= KV8_MAX_CTAS * 4 && SUMS_AT >= PLACES_AT + KV8_PLACES * 4, "a counter for each CTA, a word for each place");
+constexpr size_t COUNTERS_AT = 256, PLACES_AT = 1024, SUMS_AT = 4096;
+static_assert(PLACES_AT >= COUNTERS_AT + KV8_MAX_CTAS * 4 && SUMS_AT >= PLACES_AT + KV8_PLACES * 4, "a counter for each CTA, a word for each place");
 size_t held_bytes(const pg_kv8_cache* c, int dtype) {
   return dtype == PG_DTYPE_F32 ? ((size_t)KV8_MAX_CTAS * kv8_held(kv8_padded(c->head_dim)) * 4 + 255) / 256 * 256 : 0;
 }
@@ -197,9 +197,9 @@ int pg_kv8_attention(const pg_kv8_cache* cache, const void* q, int64_t q_row, vo
   if (window > INT32_MAX / 2) window = 0;  // wider than any table: its arithmetic stays within 32 bits
   // rows that fill less than half a tile of the portion kernel, and all of them where it has no table of rows
   const bool portions = row_start && (int64_t)group * max_rows > KV8_STEP_ROWS;
-  char* const sums = (char*)workspace + SUMS_AT;
+  char *const base = (char*)workspace, *const sums = base + SUMS_AT;
   Kv8AttnArgs a{view(cache), q, out, q_row, out_row, heads, group, rows, max_rows, row_start, lens, scale, window, window > 0 ? keep_first : 0,
-                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)workspace, (unsigned*)((char*)workspace + PLACES_AT),
+                portions ? KV8_STEP_ROWS : INT32_MAX, (unsigned*)base, (unsigned*)(base + COUNTERS_AT), (unsigned*)(base + PLACES_AT),
                 (float*)(sums + held_bytes(cache, dtype)), (float*)sums};
   if (!portions) return launched(launch_kv8_attention_step(a, dtype, scope.sms(), (cudaStream_t)stream), "kv8_attention");
   a.max_rows = std::min(max_rows, (KV8_STEP_ROWS + group - 1) / group);

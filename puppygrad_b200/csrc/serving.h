@@ -47,7 +47,7 @@ struct Kv8AttnArgs {
   float scale;
   int window, keep;
   int step_rows;  // sequences of at most so many (token, head of the group) rows are the step kernel's, the others the portion kernel's
-  unsigned *counters, *places;
+  unsigned *status, *counters, *places;
   float *partials, *held;
 };
 struct Q4Args {

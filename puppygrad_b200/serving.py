@@ -150,7 +150,8 @@ class Kv8Cache:
                   keep_first: int = 0, stream: int = 0) -> None:
         """out = softmax(scale * q . k) v over what each row sees; q and out [rows, heads, head_dim], scale head_dim ** -0.5 unless
         given, `lens` and `row_start` as in `append`. max_rows: at least the rows of any sequence. `workspace`: uint8, zeroed
-        before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each."""
+        before its first use, of workspace_bytes(); calls that may overlap on the GPU need one each. Its first 4 bytes stay zero
+        unless a wait within a kernel ran out, which leaves NaN rows."""
         device, kind, shape = self.device, q.dtype, (*_sides(q, "q", 3)[:2], self.head_dim)
         rows, heads = shape[:2]
         if (rows | heads | max_rows | window | keep_first) >> 31:

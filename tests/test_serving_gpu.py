@@ -933,3 +933,17 @@ def test_attention_long_sums_of_values_of_one_sign(seqs, rows, heads, dim, dtype
         want = ref.attention(q[some, :h].double(), k, v, torch.arange(n - rows, n, device=DEV)[:3], dim ** -0.5)
         tol = top * (2.0 ** -15 if dtype == F32 else 2.0 ** -10) + U[dtype] * want.abs()
         assert ((out[some, :h].double() - want).abs() <= tol).all(), (b, float(((out[some, :h].double() - want) / want).mean()))
+
+
+def test_attention_status_of_the_workspace():
+    """The first 32 bits: left alone by calls whose waits end, so that what an earlier call said stays until the caller zeroes it."""
+    cache = Cache([9000, 300], 2, 128, 64, 3)
+    for before in (0, 1):
+        for rows in ([1, 1], [130, 5]):
+            ws = workspace(cache, sum(rows), 4, F32)
+            ws[:4].view(torch.int32).fill_(before)
+            q = torch.randn(sum(rows), 4, 128, generator=gen(1), device=DEV)
+            out = torch.empty_like(q)
+            cache.handle.attention(q, out, i32(cache.lens), ws, row_start=starts(rows), max_rows=max(rows))
+            check_attention(cache, q, out, rows, 128 ** -0.5)
+            assert int(ws[:4].view(torch.int32)) == before
