@@ -650,9 +650,8 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
       }
       __syncthreads();
       if (last_here) {
-        // of the CTAs' parts only the first can be of a tile that began before its CTA's share
-        const bool split = at < shares.begin(first_cta);
-        auto part_of = [&](int i) { return a.partials + (size_t)((first_cta + i) * 2 + (i == 0 && !split ? 1 : 0)) * PART; };
+        // the tile begins in the first one's share, whose last tile it is, and before the others' shares
+        auto part_of = [&](int i) { return a.partials + (size_t)((first_cta + i) * 2 + (i == 0 ? 1 : 0)) * PART; };
 #pragma unroll 1
         for (int row = warp; row < t.rows; row += WARPS) {
           float top = -INFINITY, l = 0.f;
