@@ -46,16 +46,6 @@ struct Shape {
   static constexpr int SMEM = WARPS * SLOTS * SLOT;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -360,225 +350,225 @@ __global__ void __launch_bounds__(Shape<DP, NB>::THREADS, 1) kv8_step_kernel(Kv8
         }
     }
 
-      float o[MT][NB][4];
+    float o[MT][NB][4];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
-      float m[NB][2], l[NB][2];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
-
-#pragma unroll 1
-      for (int x = x0; x < x1; ++x, ++u) {
-        const int t0 = start_of(t.span, x), tok = t0 + (g >> 1) * 16 + (g & 1);  // this lane's scores: tok + 2 j, j = 0..7
-        // waits for slot i, has the one AHEAD of it sent for, and gives its place
-        auto slot = [&](int i) {
-          copy_wait<AHEAD - 1>();
-          const uint32_t from = ring + rd;
-          rd = rd == (S::SLOTS - 1) * SLOT ? 0 : rd + SLOT;
-          const int k = i + AHEAD;
-          if (k < 2 * KC) {
-            fetch(cur, k);
-          } else {
-            if (x + 1 < x1) {
-              if (k == 2 * KC) next_source(nxt);
-              fetch(nxt, k - 2 * KC);
-            }
-          }
-          copy_commit();
-          return from;
-        };
-        float s[4][NB][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][n][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < KC; ++i) {
-          const uint32_t from = slot(i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {  // tokens of rows r and r + 8: key rows 2 j and 2 j + 1 of the lane
-            const uint4 k0 = shared16(from + 2 * j * 512), k1 = shared16(from + (2 * j + 1) * 512);
-            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-            uint32_t f[4][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              f[e][0] = e4m3x2_to_f16x2(w0[e] & 0xFFFFu);
-              f[e][1] = e4m3x2_to_f16x2(w1[e] & 0xFFFFu);
-              f[e][2] = e4m3x2_to_f16x2(w0[e] >> 16);
-              f[e][3] = e4m3x2_to_f16x2(w1[e] >> 16);
-            }
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-              if constexpr (PAIR) {  // the rests first, and the sum in registers: the instruction cuts off what it adds
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], ql[n][i * 4 + e][0], ql[n][i * 4 + e][1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[j][n][e] += d[e];
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mma_f16(s[j][n], f[e][0], f[e][1], f[e][2], f[e][3], qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
-              }
-            }
-          }
-        }
-        // ---- exponents; masked ones are -infinity whatever the bytes were
-        const float sv = fmaxf(cur.scale.y, 7.888609e-31f);  // 2^-100, the least scale that an append writes
-        const bool odd = cur.scale.y != cur.scale.y;
-        const float ev = odd ? cur.scale.y : __log2f(sv), inv_v = odd ? 1.f : LOWER / sv;
-        const bool whole = __all_sync(ALL_LANES, cur.page >= 0) && t0 + UNIT - 1 <= pos_low && t0 + UNIT <= t.have &&
-                           (a.window == 0 || t0 > pos_high - a.window || t0 + UNIT <= a.keep);
-        uint32_t ph[NB][8], pl[PAIR ? NB : 1][8];
-        float down[NB][2];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          float f0 = back[n][0] * cur.scale.x, f1 = back[n][1] * cur.scale.x, add = ev;
-          if (!whole) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int k = tok + 4 * j + (e & 2), p = pos[n][e & 1];
-                const bool seen = cur.page >= 0 && k <= p && k < t.have && (a.window == 0 || k > p - a.window || k < a.keep);
-                s[j][n][e] = seen ? fmaf(s[j][n][e], e & 1 ? f1 : f0, ev) : -INFINITY;
-              }
-            f0 = f1 = 1.f;
-            add = 0.f;
-          }
-          // ---- running maximum and denominator; the maximum rounded up to a whole number, so that less the blocks' exponents it is exact
-          float raw[2] = {fmaxf(s[0][n][0], s[0][n][2]), fmaxf(s[0][n][1], s[0][n][3])};
-#pragma unroll
-          for (int j = 1; j < 4; ++j) {
-            raw[0] = fmaxf(raw[0], fmaxf(s[j][n][0], s[j][n][2]));
-            raw[1] = fmaxf(raw[1], fmaxf(s[j][n][1], s[j][n][3]));
-          }
-          float top[2] = {fmaxf(m[n][0], ceilf(__fmaf_ru(raw[0], f0, add))), fmaxf(m[n][1], ceilf(__fmaf_ru(raw[1], f1, add)))};
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            top[0] = fmaxf(top[0], __shfl_xor_sync(ALL_LANES, top[0], off));
-            top[1] = fmaxf(top[1], __shfl_xor_sync(ALL_LANES, top[1], off));
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float base = top[e] == -INFINITY ? 0.f : top[e];
-            down[n][e] = ex2(m[n][e] - base);
-            m[n][e] = top[e];
-            top[e] = __fadd_rd(__fsub_rd(add, base), WEIGHT_BITS);
-          }
-          float sum[2] = {0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[j][n][e] = ex2(fmaf(s[j][n][e], e & 1 ? f1 : f0, top[e & 1]));
-              sum[e & 1] += s[j][n][e];
-            }
-            const uint32_t h0 = pack_f16(s[j][n][0], s[j][n][1]), h1 = pack_f16(s[j][n][2], s[j][n][3]);
-            ph[n][2 * j] = transposed(h0);
-            ph[n][2 * j + 1] = transposed(h1);
-            if constexpr (PAIR) {
-              const float2 r0 = unpack_f16(h0), r1 = unpack_f16(h1);
-              pl[n][2 * j] = transposed(pack_f16(s[j][n][0] - r0.x, s[j][n][1] - r0.y));
-              pl[n][2 * j + 1] = transposed(pack_f16(s[j][n][2] - r1.x, s[j][n][3] - r1.y));
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) l[n][e] = fmaf(sum[e], inv_v, l[n][e] * down[n][e]);
-        }
-        // bytes behind the sequence's end may be anything, and 0 times NaN is NaN
-        const int live = t.have - t0 - cc * 16;
-        const bool cut = !whole && live < 16;
-#pragma unroll
-        for (int i = 0; i < KC; ++i) {
-          const uint32_t from = slot(KC + i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {  // head entries of rows r and r + 8
-            uint4 v0 = shared16(from + 2 * j * 512), v1 = shared16(from + (2 * j + 1) * 512);
-            if (cut) {
-              auto keep_bytes = [&](uint32_t& w, int k) { w = live >= k + 4 ? w : live <= k ? 0u : w & ((1u << 8 * (live - k)) - 1); };
-              keep_bytes(v0.x, 0); keep_bytes(v0.y, 4); keep_bytes(v0.z, 8); keep_bytes(v0.w, 12);
-              keep_bytes(v1.x, 0); keep_bytes(v1.y, 4); keep_bytes(v1.z, 8); keep_bytes(v1.w, 12);
-            }
-            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
-            uint32_t f[4][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              f[e][0] = e4m3x2_to_f16x2(w0[e] & 0xFFFFu);
-              f[e][1] = e4m3x2_to_f16x2(w1[e] & 0xFFFFu);
-              f[e][2] = e4m3x2_to_f16x2(w0[e] >> 16);
-              f[e][3] = e4m3x2_to_f16x2(w1[e] >> 16);
-            }
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {  // a unit's sums start from zero and join the others in registers
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              if constexpr (PAIR) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], pl[n][2 * e], pl[n][2 * e + 1]);
-              }
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], ph[n][2 * e], ph[n][2 * e + 1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[i * 4 + j][n][e] = fmaf(o[i * 4 + j][n][e], down[n][e & 1], d[e]);
-            }
-          }
-        }
-        cur = nxt;
-      }
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+    float m[NB][2], l[NB][2];
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) l[n][e] += __shfl_xor_sync(ALL_LANES, l[n][e], off);
+    for (int n = 0; n < NB; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
 
-      // ---- a tile that is complete goes out, a part of one waits for the others
-      if (x0 == 0 && x1 == t.units) {
+#pragma unroll 1
+    for (int x = x0; x < x1; ++x, ++u) {
+      const int t0 = start_of(t.span, x), tok = t0 + (g >> 1) * 16 + (g & 1);  // this lane's scores: tok + 2 j, j = 0..7
+      // waits for slot i, has the one AHEAD of it sent for, and gives its place
+      auto slot = [&](int i) {
+        copy_wait<AHEAD - 1>();
+        const uint32_t from = ring + rd;
+        rd = rd == (S::SLOTS - 1) * SLOT ? 0 : rd + SLOT;
+        const int k = i + AHEAD;
+        if (k < 2 * KC) {
+          fetch(cur, k);
+        } else {
+          if (x + 1 < x1) {
+            if (k == 2 * KC) next_source(nxt);
+            fetch(nxt, k - 2 * KC);
+          }
+        }
+        copy_commit();
+        return from;
+      };
+      float s[4][NB][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = n * 8 + cc * 2 + e, x = t.row0 + row, r = t.n_rows == 1 ? 0 : x / a.group;
-            if (row >= t.rows) continue;
-            T* to = (T*)a.out + (size_t)(t.first_row + r) * a.out_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim;
-            const float f = l[n][e] == 0.f ? 0.f : LOWER / l[n][e];
+          for (int e = 0; e < 4; ++e) s[j][n][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              if (16 * i + g < c.dim) to[16 * i + g] = from_f32<T>(o[i][n][e] * f);
-              if (16 * i + g + 8 < c.dim) to[16 * i + g + 8] = from_f32<T>(o[i][n][e + 2] * f);
+      for (int i = 0; i < KC; ++i) {
+        const uint32_t from = slot(i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // tokens of rows r and r + 8: key rows 2 j and 2 j + 1 of the lane
+          const uint4 k0 = shared16(from + 2 * j * 512), k1 = shared16(from + (2 * j + 1) * 512);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          uint32_t f[4][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[e][0] = e4m3x2_to_f16x2(w0[e] & 0xFFFFu);
+            f[e][1] = e4m3x2_to_f16x2(w1[e] & 0xFFFFu);
+            f[e][2] = e4m3x2_to_f16x2(w0[e] >> 16);
+            f[e][3] = e4m3x2_to_f16x2(w1[e] >> 16);
+          }
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            if constexpr (PAIR) {  // the rests first, and the sum in registers: the instruction cuts off what it adds
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], ql[n][i * 4 + e][0], ql[n][i * 4 + e][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[j][n][e] += d[e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mma_f16(s[j][n], f[e][0], f[e][1], f[e][2], f[e][3], qh[n][i * 4 + e][0], qh[n][i * 4 + e][1]);
             }
           }
-      } else {
-        __syncwarp();  // all lanes have read their last bytes of the ring
-        float* w = u == u1 ? last_part(warp) : early_part(warp);
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = n * 8 + cc * 2 + e;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              w[row * DP + 16 * i + g] = o[i][n][e];
-              w[row * DP + 16 * i + g + 8] = o[i][n][e + 2];
-            }
-            if (g == 0) {
-              w[ROWS * DP + row] = m[n][e];
-              w[ROWS * (DP + 1) + row] = l[n][e];
-            }
-          }
-        if (lane == 0) {
-          part_tile[warp * 2 + (u == u1 ? 1 : 0)] = t.first_unit;
-          part_of_tile[warp * 2 + (u == u1 ? 1 : 0)] = t;
         }
       }
-      copy_wait<0>();  // (nothing but empty groups)
+      // ---- exponents; masked ones are -infinity whatever the bytes were
+      const float sv = fmaxf(cur.scale.y, 7.888609e-31f);  // 2^-100, the least scale that an append writes
+      const bool odd = cur.scale.y != cur.scale.y;
+      const float ev = odd ? cur.scale.y : __log2f(sv), inv_v = odd ? 1.f : LOWER / sv;
+      const bool whole = __all_sync(ALL_LANES, cur.page >= 0) && t0 + UNIT - 1 <= pos_low && t0 + UNIT <= t.have &&
+                         (a.window == 0 || t0 > pos_high - a.window || t0 + UNIT <= a.keep);
+      uint32_t ph[NB][8], pl[PAIR ? NB : 1][8];
+      float down[NB][2];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        float f0 = back[n][0] * cur.scale.x, f1 = back[n][1] * cur.scale.x, add = ev;
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = tok + 4 * j + (e & 2), p = pos[n][e & 1];
+              const bool seen = cur.page >= 0 && k <= p && k < t.have && (a.window == 0 || k > p - a.window || k < a.keep);
+              s[j][n][e] = seen ? fmaf(s[j][n][e], e & 1 ? f1 : f0, ev) : -INFINITY;
+            }
+          f0 = f1 = 1.f;
+          add = 0.f;
+        }
+        // ---- running maximum and denominator; the maximum rounded up to a whole number, so that less the blocks' exponents it is exact
+        float raw[2] = {fmaxf(s[0][n][0], s[0][n][2]), fmaxf(s[0][n][1], s[0][n][3])};
+#pragma unroll
+        for (int j = 1; j < 4; ++j) {
+          raw[0] = fmaxf(raw[0], fmaxf(s[j][n][0], s[j][n][2]));
+          raw[1] = fmaxf(raw[1], fmaxf(s[j][n][1], s[j][n][3]));
+        }
+        float top[2] = {fmaxf(m[n][0], ceilf(__fmaf_ru(raw[0], f0, add))), fmaxf(m[n][1], ceilf(__fmaf_ru(raw[1], f1, add)))};
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(ALL_LANES, top[0], off));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(ALL_LANES, top[1], off));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float base = top[e] == -INFINITY ? 0.f : top[e];
+          down[n][e] = ex2(m[n][e] - base);
+          m[n][e] = top[e];
+          top[e] = __fadd_rd(__fsub_rd(add, base), WEIGHT_BITS);
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[j][n][e] = ex2(fmaf(s[j][n][e], e & 1 ? f1 : f0, top[e & 1]));
+            sum[e & 1] += s[j][n][e];
+          }
+          const uint32_t h0 = pack_f16(s[j][n][0], s[j][n][1]), h1 = pack_f16(s[j][n][2], s[j][n][3]);
+          ph[n][2 * j] = transposed(h0);
+          ph[n][2 * j + 1] = transposed(h1);
+          if constexpr (PAIR) {
+            const float2 r0 = unpack_f16(h0), r1 = unpack_f16(h1);
+            pl[n][2 * j] = transposed(pack_f16(s[j][n][0] - r0.x, s[j][n][1] - r0.y));
+            pl[n][2 * j + 1] = transposed(pack_f16(s[j][n][2] - r1.x, s[j][n][3] - r1.y));
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[n][e] = fmaf(sum[e], inv_v, l[n][e] * down[n][e]);
+      }
+      // bytes behind the sequence's end may be anything, and 0 times NaN is NaN
+      const int live = t.have - t0 - cc * 16;
+      const bool cut = !whole && live < 16;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const uint32_t from = slot(KC + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // head entries of rows r and r + 8
+          uint4 v0 = shared16(from + 2 * j * 512), v1 = shared16(from + (2 * j + 1) * 512);
+          if (cut) {
+            auto keep_bytes = [&](uint32_t& w, int k) { w = live >= k + 4 ? w : live <= k ? 0u : w & ((1u << 8 * (live - k)) - 1); };
+            keep_bytes(v0.x, 0); keep_bytes(v0.y, 4); keep_bytes(v0.z, 8); keep_bytes(v0.w, 12);
+            keep_bytes(v1.x, 0); keep_bytes(v1.y, 4); keep_bytes(v1.z, 8); keep_bytes(v1.w, 12);
+          }
+          const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+          uint32_t f[4][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[e][0] = e4m3x2_to_f16x2(w0[e] & 0xFFFFu);
+            f[e][1] = e4m3x2_to_f16x2(w1[e] & 0xFFFFu);
+            f[e][2] = e4m3x2_to_f16x2(w0[e] >> 16);
+            f[e][3] = e4m3x2_to_f16x2(w1[e] >> 16);
+          }
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {  // a unit's sums start from zero and join the others in registers
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (PAIR) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], pl[n][2 * e], pl[n][2 * e + 1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_f16(d, f[e][0], f[e][1], f[e][2], f[e][3], ph[n][2 * e], ph[n][2 * e + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i * 4 + j][n][e] = fmaf(o[i * 4 + j][n][e], down[n][e & 1], d[e]);
+          }
+        }
+      }
+      cur = nxt;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][e] += __shfl_xor_sync(ALL_LANES, l[n][e], off);
+
+    // ---- a tile that is complete goes out, a part of one waits for the others
+    if (x0 == 0 && x1 == t.units) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = n * 8 + cc * 2 + e, x = t.row0 + row, r = t.n_rows == 1 ? 0 : x / a.group;
+          if (row >= t.rows) continue;
+          T* to = (T*)a.out + (size_t)(t.first_row + r) * a.out_row + (size_t)(t.head * a.group + (x - r * a.group)) * c.dim;
+          const float f = l[n][e] == 0.f ? 0.f : LOWER / l[n][e];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            if (16 * i + g < c.dim) to[16 * i + g] = from_f32<T>(o[i][n][e] * f);
+            if (16 * i + g + 8 < c.dim) to[16 * i + g + 8] = from_f32<T>(o[i][n][e + 2] * f);
+          }
+        }
+    } else {
+      __syncwarp();  // all lanes have read their last bytes of the ring
+      float* w = u == u1 ? last_part(warp) : early_part(warp);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = n * 8 + cc * 2 + e;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            w[row * DP + 16 * i + g] = o[i][n][e];
+            w[row * DP + 16 * i + g + 8] = o[i][n][e + 2];
+          }
+          if (g == 0) {
+            w[ROWS * DP + row] = m[n][e];
+            w[ROWS * (DP + 1) + row] = l[n][e];
+          }
+        }
+      if (lane == 0) {
+        part_tile[warp * 2 + (u == u1 ? 1 : 0)] = t.first_unit;
+        part_of_tile[warp * 2 + (u == u1 ? 1 : 0)] = t;
+      }
+    }
+    copy_wait<0>();  // (nothing but empty groups)
   }
   __syncthreads();  // parts in global memory too are read by this block alone
 
