@@ -947,3 +947,55 @@ def test_attention_status_of_the_workspace():
             cache.handle.attention(q, out, i32(cache.lens), ws, row_start=starts(rows), max_rows=max(rows))
             check_attention(cache, q, out, rows, 128 ** -0.5)
             assert int(ws[:4].view(torch.int32)) == before
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_sums_in_memory_of_more_blocks_than_run_at_once(dim):
+    """FP32 portions long enough for sums in memory, more of them than there are places for those: all sequences alike, so all results alike."""
+    n, seqs, rows, heads, page = 3000, 450, 2, 64, 64
+    one = Cache([n], 1, dim, page, 5)
+    one.table = one.table.repeat(seqs, 1)
+    one.handle = pg.Kv8Cache(one.pool, one.scales, one.table, page_tokens=page, head_dim=dim)
+    q = torch.randn(rows, heads, dim, generator=gen(2), device=DEV).repeat(seqs, 1, 1)
+    out = torch.full_like(q, 1e4)
+    one.handle.attention(q, out, i32([n] * seqs), workspace(one, seqs * rows, heads, F32), row_start=starts([rows] * seqs), max_rows=rows)
+    check_attention(one, q[:rows], out[:rows], [rows], dim ** -0.5)
+    assert (out.view(seqs, -1) == out[:rows].reshape(1, -1)).all()
+
+
+@pytest.mark.parametrize("window,keep,gone", [(0, 0, 2600), (2600, 2400, 0), (4500, 100, 7000)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_portions_whose_first_pieces_are_not_seen(window, keep, gone, dtype):
+    """Pieces of which a row sees nothing come first: on no page, or kept for other rows."""
+    n, rows, heads = 9000, 150, 4
+    cache = Cache([n], 2, 64, 64, 9)
+    cache.table[0, :gone // 64] = -1
+    q = torch.randn(rows, heads, 64, generator=gen(4), device=DEV).to(dtype)
+    out = torch.full_like(q, 1e4)
+    cache.handle.attention(q, out, i32([n]), workspace(cache, rows, heads, dtype), row_start=starts([rows]), max_rows=rows, window=window, keep_first=keep)
+    cache.table.clamp_(min=0)
+    keys, values = cache.kv(0)
+    want = ref.attention(q.double(), keys, values, torch.arange(n - rows, n, device=DEV), 0.125, window, keep, missing=torch.arange(n, device=DEV) < gone // 64 * 64)
+    tol = float(values.abs().max()) * (2.0 ** -15 if dtype == F32 else 2.0 ** -10) + U[dtype] * want.abs()
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_append_at_far_positions(rows, dtype):
+    """Angles of positions around a million, of the tokens and of the queries."""
+    page, dim, heads, length = 64, 64, 2, 1000000
+    pages = 3
+    pool = torch.zeros(pg.Kv8Cache.pool_shape(pages, 1, page, dim), dtype=torch.uint8, device=DEV)
+    table = torch.full((1, -(-length // page)), -1, dtype=torch.int32, device=DEV)
+    table[0, -pages:] = torch.arange(pages, dtype=torch.int32, device=DEV)
+    cache = pg.Kv8Cache(pool, torch.zeros(pages, 1, 2, device=DEV), table, page_tokens=page, head_dim=dim)
+    q, k = (torch.randn(rows, h, dim, generator=gen(h), device=DEV).to(dtype) for h in (heads, 1))
+    out = torch.empty_like(q)
+    cache.append(k, k, i32([length]), row_start=None if rows == 1 else starts([rows]), q=q, q_out=out, rot_dims=dim)
+    pos = torch.arange(length - rows, length, device=DEV)
+    want = ref.rotate(q.double(), pos, dim, 10000.0)
+    assert ((out.double() - want).abs() <= U[dtype] * want.abs() + 2.0 ** -22 * q.double().abs().amax(-1, keepdim=True)).all()
+    keys, _ = ref.sequence_kv(pool, cache.scales, table[0, -pages:], pages * page, page, dim)
+    held, want = keys[-rows:], ref.rotate(k.double(), pos, dim, 10000.0)  # the last page is full
+    assert ((held - want).abs() <= 0.07 * want.abs() + 1e-2).all()
