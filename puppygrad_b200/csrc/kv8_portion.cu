@@ -7,7 +7,7 @@
 // so both are K-major as they come. Four softmax warps for each tile have a row for every thread, which needs no exchange between
 // threads; one warp issues the products, the scores of a piece in front of the values of the one before it, so that the tensor pipe
 // works while the softmax of the next scores is computed. Two tiles share the producers' work at head_dim 128 (1500 rows behind 2600
-// positions of two sequences, 32 query heads: 237 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are
+// positions of two sequences, 32 query heads: 238 us, 282 us with one tile a CTA and two CTAs an SM); at 64 two CTAs with a tile each are
 // better (1000 rows of four sequences, 12 heads: 42 us, 55 us), above 128 tensor memory has room for one.
 // The instruction cuts off what it adds to O, up to 5*10^-8 of it each time, and always towards zero, so that sums of one sign drift: 4*10^-4 over 65536
 // positions of FP32 rows. Theirs therefore join sums in memory (a place of the workspace for each CTA that is running) after every 32 pieces, by rounded
@@ -18,13 +18,13 @@
 //
 // Scales, weights and the running maximum are those of the step kernel: the value scale is part of the exponent, the denominator
 // divides it out. The maximum that weights refer to (a whole number: less the blocks' exponents it is exact) moves only when a row
-// outgrows it by 2^3, which spares most passes over O; weights are up to 2^12 there, which leaves those to FP16's range. FP32 rows are pairs of FP16 numbers, queries and weights alike:
-// two products into the same accumulator.
+// outgrows it by 2^3, which spares most passes over O; weights are up to 2^12 there, which leaves those to FP16's range. FP32 rows are pairs
+// of FP16 numbers, queries and weights alike: two products into the same accumulator.
 //
 // Bound: 64 exponentials for every 64 * 2 * head_dim multiply-adds of a row keep the special-function and the tensor pipe equally busy at
 // head_dim 128, 1024 cycles for 256 rows and 64 positions. Measured there: 2700 cycles. A softmax warp takes 400 for the maximum, 250 to
-// get the scores, 1200 for exponentials, sums and stores, and two of them share a scheduler and its special functions; 0.6 PFLOP/s, 237 us
-// for the portions above, 452 us with FP32 rows. Three producer warps are too few at 128 (321 us), seven no better than four (249 us);
+// get the scores, 1200 for exponentials, sums and stores, and two of them share a scheduler and its special functions; 0.6 PFLOP/s, 238 us
+// for the portions above (384 CTAs, so that an SM is active for four fifths of it), 449 us with FP32 rows. Three producer warps are too few at 128 (321 us), seven no better than four (249 us);
 // above 128 eight are better than four (head_dim 256, 1000 rows of four sequences: 158 us, 168 us).
 #include <algorithm>
 #include <type_traits>
@@ -89,7 +89,8 @@ __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.
 // there are no sums (any = false) the rows get `fill`, and that memory, which may still be in use, is left alone. `held` (or null): more sums of this thread's
 // row, a column every `step`, to be multiplied with f.
 template <typename E, int COLS, typename F>
-__device__ __forceinline__ void rows_out(uint8_t* mine, uint32_t taddr, bool any, float fill, const float* held, int step, float f, float by, int dim, bool wide, F to) {
+__device__ __forceinline__ void rows_out(uint8_t* mine, uint32_t taddr, bool any, float fill, const float* held, int step, float f, float by, int dim,
+                                         bool wide, F to) {
   constexpr int PER = 16 / sizeof(E), VECS = COLS / PER;
   static_assert(VECS % 8 == 0, "places are swapped among eight");
   const int lane = threadIdx.x & 31;
@@ -410,7 +411,8 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
         if (i < rows) *reinterpret_cast<float2*>(to + (size_t)TILES * ROWS * DP + 2 * i) = make_float2(m_ref, sum);
 #pragma unroll 1
         for (int d = 0; d < DP; d += DP / 2)
-          rows_out<float, DP / 2>(mine, tmem_o + d, any, fill, more ? more + d * NEXT : nullptr, NEXT, f, 1.f, DP / 2, true, [&](int k) { return row_w + k < rows ? to + (row_w + k) * DP + d : nullptr; });
+          rows_out<float, DP / 2>(mine, tmem_o + d, any, fill, more ? more + d * NEXT : nullptr, NEXT, f, 1.f, DP / 2, true,
+                                  [&](int k) { return row_w + k < rows ? to + (row_w + k) * DP + d : nullptr; });
       } else {
         const int64_t at = (int64_t)(r.first + tok) * a.out_row + entry;
         rows_out<T, DP>(mine, tmem_o, any, fill, more, NEXT, f, sum == 0.f ? 0.f : LOWER / sum, c.dim, wide_of(a.out, a.out_row), [&](int k) {
@@ -467,7 +469,8 @@ __global__ void __launch_bounds__(PortionShape<DP, T>::THREADS, PortionShape<DP,
             for (int p = PAIR ? 1 : 0; p >= 0; --p)
 #pragma unroll
               for (int k = 0; k < TOKENS / 16; ++k)
-                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o, (PAIR ? j % S::KEEP : j) != 0 || p != (PAIR ? 1 : 0) || k != 0);
+                umma_bf16_ts(to, from + (uint32_t)((k >> 1) * 32 + p * 16 + (k & 1) * 8), dv + (uint32_t)(k * 2), idesc_o,
+                             (PAIR ? j % S::KEEP : j) != 0 || p != (PAIR ? 1 : 0) || k != 0);
             umma_commit(&o_done[t]);
             if (t == tiles - 1) umma_commit(&empty[now.stage]);
           }

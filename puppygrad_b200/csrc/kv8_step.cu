@@ -17,12 +17,14 @@
 // log2 scale_v - m), so that O = sum w code and the weights stay within [0, 1] however the scales differ; the denominator adds w /
 // scale_v. m is the running maximum of that exponent, rounded up, less 15: FP16 holds up to 2^16, and what rounds to nothing at its lower end
 // is then below 2^-40 of the largest. FP32 queries and their weights are pairs of FP16 numbers, two instructions into one accumulator: FP32
-// grade. Rounding: BF16 queries are exact in FP16 after their row's scaling to [1, 2), their weights round to FP16 (2^-11 of each).
+// grade. Rounding: BF16 queries are exact in FP16 after their row's scaling to [1, 2) (entries below 2^-17 of the largest: to 2^-25 of it), their weights
+// round to FP16 (2^-11 of each).
 //
-// Bound: memory, at HBM's rate while bytes are on their way. Beside them a call takes the start (units counted, page table, scales: 4300
-// cycles until the first bytes are asked for), the SMs' different speeds (equal shares end 20% apart) and the merges (10000 cycles where
-// tiles are cut). Measured: 64 sequences, 32 query and 8 key / value heads of 128: 71 us for 202 MB (31 by bytes); two sequences of 131000
-// positions 67 us (41); one of 777 10.8 us; 64 FP32 rows 82 us.
+// Bound by bytes: 31 us for 64 sequences with 32 query and 8 key / value heads of 128 (202 MB). Measured: 71 us, 135000 cycles, of which an SM is active
+// 100000 on average, 126000 at most: equal shares end a quarter apart. Of its time an SM takes 4300 cycles until it asks for the first bytes (units
+// counted, page table, scales) and 10000 to merge cut tiles; the 85000 in between are half as many again as HBM's rate would need, for a reason that is
+// not established (schedulers issue in 32 of 100 cycles and wait for bytes, at the end for other warps). Two sequences of 131000 positions 68 us
+// (41 by bytes), one of 777 10.9 us, 64 FP32 rows 81 us.
 #include <algorithm>
 #include <type_traits>
 

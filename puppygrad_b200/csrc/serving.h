@@ -9,9 +9,15 @@
 namespace pg {
 
 constexpr int KV8_MAX_SEQS = 4096;
-// Rows of a (sequence, head) up to which the step kernel has them. us, step / portion kernel, at 32, 48 and 64 rows: 16 sequences of 2000
-// positions, 8 heads of 128, BF16 49 / 51, 65 / 50, 77 / 50, FP32 76 / 71, 104 / 72, 131 / 72; 64 of them BF16 140 / 229, 197 / 232, 254 / 261, FP32
-// 269 / 290, 387 / 302, 513 / 312; 12 heads of 64 BF16 137 / 180, 176 / 185, 241 / 201; 8 of 4000, 4 heads of 256, BF16 64 / 59, 88 / 69, 106 / 70.
+// Rows of a (sequence, head) up to which the step kernel has them. us, step / portion kernel:
+//   rows                                    16         32         40         48         64
+//   16 sequences of 2000, 8 heads of 128,   38 / 47    50 / 49    64 / 51    65 / 51    78 / 51     FP32  49 / 70    73 / 72    88 / 72    101 / 73   127 / 73
+//   64 of them                              83 / 214   142 / 229  198 / 229  202 / 230  252 / 232   FP32  145 / 271  262 / 288  306 / 288  376 / 288  492 / 290
+//   64 of 2000, 12 heads of 64              77 / 170   135 / 179  173 / 180  174 / 180  238 / 182   FP32  107 / 192  182 / 202  211 / 202  251 / 203  306 / 205
+//   one of 8000, 8 heads of 128             20 / 38    23 / 41    28 / 41    28 / 41    32 / 42     FP32  22 / 49    29 / 51    35 / 51    35 / 51    43 / 51
+//   8 of 4000, 4 heads of 256               45 / 53    62 / 57    73 / 59    84 / 67    101 / 70    FP32  55 / 85    76 / 89    89 / 89    103 / 108  124 / 111
+// The two cross between 32 and 64 rows, at other places for other loads (and not yet for a single sequence). One number for all of them: at
+// 40 rows up to a quarter is lost (16 sequences), at 48 a seventh (64 BF16 sequences), half as much again as the step kernel's time for a single one.
 constexpr int KV8_STEP_ROWS = 40;
 constexpr int KV8_MAX_CTAS = 160;  // of the step kernel's persistent grid: the size of its workspace does not hang on the device
 constexpr int KV8_PLACES = 2 * KV8_MAX_CTAS;  // for sums in memory of CTAs of the portion kernel, of which two run on an SM at head_dim 64

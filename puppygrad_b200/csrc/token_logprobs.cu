@@ -5,9 +5,11 @@
 // row: the k-th largest of the threads' maxima, tau, is a lower bound of the k-th largest entry, and every entry from tau on was met by
 // one of the k threads whose maxima are the largest, so only what those k threads met is read again (from L2). Entries are ordered by
 // (value, lower id first) as one 64-bit key, which makes the order total and the k threads unambiguous.
-// Bound: memory; in BF16 one exponential for two bytes keeps the special-function units three quarters busy at that rate, so the rest
-// is kept to a few instructions: maximum and minimum of two entries at once, multiply-adds of two at once. Entries that are masked
-// (-infinity, the type's lowest value) would give 0 * infinity in U: where a batch has one so low, its exponents are clamped.
+// Bound: bytes, 40 us for 4096 x 32000 BF16 and 80 in FP32; measured 53 (schedulers issue in 74 of 100 cycles, the special functions are busy in 61)
+// and 85. In BF16 one exponential for two bytes takes 30 us of the special functions, so the rest is kept to a few instructions: maximum and
+// minimum of two entries at once, multiply-adds of two at once. Entries that are masked (-infinity, the type's lowest value) would
+// give 0 * infinity in U: where a batch has one so low, its exponents are clamped. Alternatives are the expensive part: sorts and merges of a row's candidates
+// across lanes, 17 us for five of each of those rows; 37000 x 1000 FP32 with 20 takes 195 us, 24 by bytes.
 // A row is a warp's where there are many rows (no barriers, and every SM has dozens of rows on their way), four warps' where there are
 // fewer, a block's or a cluster of up to 8 blocks' where they are few.
 #include <cfloat>
@@ -393,8 +395,8 @@ cudaError_t run(const LogprobArgs& a, int sms, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  // Measured, us with a warp / four warps / a block for a row: 37000 x 3400 BF16 64 / 99 / 385, 8000 x 8000 FP32 74 / 75 / 207,
-  // 3000 x 20000 BF16 59 / 48 / 97, 1200 x 50257 FP32 127 / 51 / 69, 500 x 30000 BF16 39 / 25 / 22, 400 x 160000 FP32 719 / 133 / 71.
+  // Measured, us with a warp / four warps / a block for a row: 37000 x 3400 BF16 64 / 99 / 385; with five alternatives 8000 x 8000 FP32 74 / 75 / 207,
+  // 3000 x 20000 BF16 59 / 48 / 97, 1200 x 50257 FP32 127 / 51 / 69, 500 x 30000 BF16 39 / 25 / 22; with 20 400 x 160000 FP32 719 / 133 / 71.
   if (a.rows >= 12 * sms && (int64_t)a.vocab * (int)sizeof(T) <= 16384) {
     cfg.gridDim = dim3((a.rows + 7) / 8);
     cfg.blockDim = dim3(256);
